@@ -36,6 +36,8 @@ SYMBOLS = [
     "fitre_select_column_matrix", "fitre_prepare_minibatch", "fitre_generalization_mem_required",
     "fitre_compute_generalization_errors", "fitre_trust_region_kfac_mem_required",
     "fitre_subsampled_trust_region_kfac", "fitre_write_vector", "fitre_read_vector",
+    "fitre_layer_norm_forward", "fitre_layer_norm_backward_mem_required", "fitre_layer_norm_backward",
+    "fitre_token_logprobs", "fitre_token_logprobs_backward",
 ]
 
 _lib = None
@@ -139,5 +141,10 @@ def load():
         C.POINTER(S.TR_EPOCH))
     sig("fitre_write_vector", i, C.c_char_p, vp, l, i)
     sig("fitre_read_vector", i, C.c_char_p, vp, l, C.POINTER(C.c_long))
+    sig("fitre_layer_norm_forward", i, vp, i, i, vp, l, vp, vp, vp, l, vp, vp, l, l, d)
+    sig("fitre_layer_norm_backward_mem_required", l, l, l)
+    sig("fitre_layer_norm_backward", i, vp, i, i, vp, l, vp, l, vp, vp, vp, vp, l, vp, vp, l, l, vp)
+    sig("fitre_token_logprobs", i, vp, i, vp, l, vp, l, l, vp, vp, vp, i, vp, vp)
+    sig("fitre_token_logprobs_backward", i, vp, i, vp, l, vp, vp, vp, vp, vp, vp, l, l, l)
     _lib = L
     return L

@@ -14,6 +14,7 @@ MODEL_TRAIN = 10
 ACT_LOGISTIC, ACT_TANH, ACT_LINEAR = 1, 2, 3
 CNN_ACT_NONE, CNN_ACT_SOFTPLUS, CNN_ACT_ELU, CNN_ACT_RELU, CNN_ACT_SWISH = 10, 11, 12, 13, 14
 MAX_POOL, AVG_POOL, NO_POOL = 0, 1, 2
+DTYPE_F64, DTYPE_F32, DTYPE_BF16, DTYPE_F16 = range(4)
 
 # status codes
 OK, ERR_BAD_ARG, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_CUDA, ERR_COMM, ERR_NOT_CONVERGED, ERR_TOO_LARGE, ERR_NOT_FINITE = range(9)

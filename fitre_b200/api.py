@@ -507,3 +507,150 @@ def readVector(path, n):
     if rc:
         raise OSError("fitre_read_vector failed for %s" % path)
     return a[:got.value]
+
+
+# ---- language-model operators ---------------------------------------------------------------
+# Matrices are 2-D CUDA tensors with unit column stride and any row stride (float64, float32,
+# bfloat16, float16); outputs are tensors of the caller's.  Everything is queued on the context's
+# stream.  See include/fitre_b200.h for the formulas and the treatment of special values.
+
+_DTYPES = {}
+
+
+def _dtype_code(t):
+    if not _DTYPES:
+        import torch
+        _DTYPES.update({torch.float64: S.DTYPE_F64, torch.float32: S.DTYPE_F32,
+                        torch.bfloat16: S.DTYPE_BF16, torch.float16: S.DTYPE_F16})
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise FitreError(S.ERR_UNSUPPORTED, "element type %s" % t.dtype)
+    return code
+
+
+def _on(ctx, t, what):
+    if not t.is_cuda or t.get_device() != ctx.device:
+        raise FitreError(S.ERR_BAD_ARG, "%s must be a tensor on CUDA device %d" % (what, ctx.device))
+
+
+def _matrix(ctx, t, what, shape=None, dtype=None):
+    """(pointer, row stride) of a matrix argument after its checks."""
+    _on(ctx, t, what)
+    if t.dim() != 2 or (shape is not None and tuple(t.shape) != shape):
+        raise FitreError(S.ERR_BAD_ARG, "%s must have shape %s" % (what, "(rows, cols)" if shape is None else shape))
+    if dtype is not None and t.dtype != dtype:
+        raise FitreError(S.ERR_BAD_ARG, "%s must be %s" % (what, dtype))
+    rows, cols = t.shape
+    s0, s1 = t.stride()
+    if cols > 1 and s1 != 1:
+        raise FitreError(S.ERR_BAD_ARG, "%s must have contiguous rows" % what)
+    return t.data_ptr(), s0 if rows > 1 else cols
+
+
+def _vector(ctx, t, what, n, dtype):
+    if t is None:
+        return None
+    _on(ctx, t, what)
+    if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+        raise FitreError(S.ERR_BAD_ARG, "%s must be contiguous, of %d elements of %s" % (what, n, dtype))
+    return t.data_ptr()
+
+
+def _scratch(ctx, t, need):
+    if t is None:
+        if need:
+            raise FitreError(S.ERR_WORKSPACE, "scratch of %d doubles needed, none given" % need)
+        return None
+    import torch
+    _on(ctx, t, "devPtr")
+    if t.dtype != torch.float64 or not t.is_contiguous():
+        raise FitreError(S.ERR_BAD_ARG, "device buffers must be contiguous float64 CUDA tensors")
+    if t.numel() < need:
+        raise FitreError(S.ERR_WORKSPACE, "scratch of %d doubles needed, %d given" % (need, t.numel()))
+    return t.data_ptr()
+
+
+def _stat(t):
+    import torch
+    return torch.float64 if t.dtype == torch.float64 else torch.float32
+
+
+def _weight_dtype(t, x):
+    import torch
+    if t is None:
+        return x.dtype
+    if t.dtype != x.dtype and (t.dtype != torch.float32 or x.dtype == torch.float64):
+        raise FitreError(S.ERR_UNSUPPORTED, "weights of %s next to %s" % (t.dtype, x.dtype))
+    return t.dtype
+
+
+def layerNormForward(ctx, x, gamma, beta, y, mean=None, rstd=None, eps=1e-5):
+    """y = (x - mean) * rstd * gamma + beta per row; mean / rstd are kept for layerNormBackward.
+    gamma / beta may be None; y may be x."""
+    code = _dtype_code(x)
+    xp, ldx = _matrix(ctx, x, "x")
+    rows, cols = x.shape
+    yp, ldy = _matrix(ctx, y, "y", (rows, cols), x.dtype)
+    w = _weight_dtype(gamma if gamma is not None else beta, x)
+    stat = _stat(x)
+    ctx.check(ctx.lib.fitre_layer_norm_forward(
+        ctx.h, code, _DTYPES[w], xp, ldx, _vector(ctx, gamma, "gamma", cols, w), _vector(ctx, beta, "beta", cols, w),
+        yp, ldy, _vector(ctx, mean, "mean", rows, stat), _vector(ctx, rstd, "rstd", rows, stat), rows, cols, eps))
+
+
+def layerNormBackwardMemRequired(rows, cols):
+    """Scratch (doubles) of layerNormBackward when dgamma or dbeta is wanted."""
+    return int(_lib.load().fitre_layer_norm_backward_mem_required(rows, cols))
+
+
+def layerNormBackward(ctx, dy, x, gamma, mean, rstd, dx, dgamma=None, dbeta=None, devPtr=None):
+    """dx, and dgamma / dbeta summed over the rows, from layerNormForward's mean and rstd."""
+    code = _dtype_code(x)
+    xp, ldx = _matrix(ctx, x, "x")
+    rows, cols = x.shape
+    dyp, lddy = _matrix(ctx, dy, "dy", (rows, cols), x.dtype)
+    dxp, lddx = _matrix(ctx, dx, "dx", (rows, cols), x.dtype)
+    given = next((t for t in (gamma, dgamma, dbeta) if t is not None), None)
+    w = _weight_dtype(given, x)
+    stat = _stat(x)
+    need = layerNormBackwardMemRequired(rows, cols) if dgamma is not None or dbeta is not None else 0
+    ctx.check(ctx.lib.fitre_layer_norm_backward(
+        ctx.h, code, _DTYPES[w], dyp, lddy, xp, ldx, _vector(ctx, gamma, "gamma", cols, w),
+        _vector(ctx, mean, "mean", rows, stat), _vector(ctx, rstd, "rstd", rows, stat), dxp, lddx,
+        _vector(ctx, dgamma, "dgamma", cols, w), _vector(ctx, dbeta, "dbeta", cols, w), rows, cols,
+        _scratch(ctx, devPtr, need)))
+
+
+def tokenLogProbs(ctx, logits, tokens, logprobs=None, lse=None, entropy=None, topLogprobs=None, topTokens=None):
+    """Per row of logits: log p(token), log sum exp, entropy, and (topLogprobs / topTokens of shape
+    (rows, top), top <= 32) the largest alternatives, lower index first among equals."""
+    import torch
+    code = _dtype_code(logits)
+    xp, ld = _matrix(ctx, logits, "logits")
+    rows, vocab = logits.shape
+    stat = _stat(logits)
+    top = 0
+    if topLogprobs is not None or topTokens is not None:
+        if topLogprobs is None or topTokens is None or topTokens.dim() != 2:
+            raise FitreError(S.ERR_BAD_ARG, "topLogprobs and topTokens go together, of shape (rows, top)")
+        top = topTokens.shape[1]
+    ctx.check(ctx.lib.fitre_token_logprobs(
+        ctx.h, code, xp, ld, _vector(ctx, tokens, "tokens", rows, torch.int64), rows, vocab,
+        _vector(ctx, logprobs, "logprobs", rows, stat), _vector(ctx, lse, "lse", rows, stat),
+        _vector(ctx, entropy, "entropy", rows, stat), top,
+        _vector(ctx, topLogprobs, "topLogprobs", rows * top, stat),
+        _vector(ctx, topTokens, "topTokens", rows * top, torch.int64)))
+
+
+def tokenLogProbsBackward(ctx, logits, tokens, lse, entropy, dLogprobs, dEntropy, dLogits):
+    """dLogits from the gradients of tokenLogProbs' logprobs and / or entropy; dLogits may be logits."""
+    import torch
+    code = _dtype_code(logits)
+    xp, ld = _matrix(ctx, logits, "logits")
+    rows, vocab = logits.shape
+    dp, ldd = _matrix(ctx, dLogits, "dLogits", (rows, vocab), logits.dtype)
+    stat = _stat(logits)
+    ctx.check(ctx.lib.fitre_token_logprobs_backward(
+        ctx.h, code, xp, ld, _vector(ctx, tokens, "tokens", rows, torch.int64), _vector(ctx, lse, "lse", rows, stat),
+        _vector(ctx, entropy, "entropy", rows, stat), _vector(ctx, dLogprobs, "dLogprobs", rows, stat),
+        _vector(ctx, dEntropy, "dEntropy", rows, stat), dp, ldd, rows, vocab))

@@ -653,6 +653,54 @@ int fitre_set_host_results_shared(fitre_context *ctx, int on);
  * ncclAllGather. */
 int fitre_set_host_inputs_replicated(fitre_context *ctx, int on);
 
+/* ---- language-model operators ------------------------------------------------------------
+ * The counterparts, for training and scoring language models, of the batch norm, activation,
+ * soft-max loss and per-layer preconditioning above.  No counterpart in the reference.  Matrices
+ * are row-major with `ld*` elements from one row to the next (>= the width; rows need no
+ * particular alignment beyond their element's, 16-byte aligned rows are fastest); element types
+ * are FITRE_DTYPE_*.  Statistics (mean, rstd, log probabilities, lse, entropy) are fp32, or fp64
+ * next to fp64 tensors, and every sum is held in that type.  Calls only queue work on the context's
+ * stream, never wait, leave the caller's current device as it was, may be captured into a CUDA
+ * graph, and give the same bits every time.  Zero rows are allowed and touch nothing but sums over
+ * rows, which are zero.  devPtr arguments are scratch in doubles, as above, 16-byte aligned; two
+ * calls that may overlap in time need scratch of their own. */
+enum { FITRE_DTYPE_F64 = 0, FITRE_DTYPE_F32 = 1, FITRE_DTYPE_BF16 = 2, FITRE_DTYPE_F16 = 3 };
+
+/* Layer norm of each row: y = (x - mean) * rstd * gamma + beta, rstd = 1 / sqrt(variance + eps).
+ * gamma / beta (cols elements, may be NULL = 1 / 0) have type `wtype`: dtype, or FITRE_DTYPE_F32 next to
+ * a 16-bit dtype.  mean / rstd (rows, may be NULL) are what the backward pass wants.  y may be x
+ * (same pointer and stride). */
+int fitre_layer_norm_forward(fitre_context *ctx, int dtype, int wtype, const void *x, long ldx,
+                             const void *gamma, const void *beta, void *y, long ldy, void *mean,
+                             void *rstd, long rows, long cols, real eps);
+/* Its gradients: dx, and dgamma / dbeta (may be NULL) summed over all rows in a fixed order.  dx may be
+ * dy or x (same pointer and stride).  devPtr: fitre_layer_norm_backward_mem_required doubles, may be NULL
+ * when neither dgamma nor dbeta is wanted. */
+long fitre_layer_norm_backward_mem_required(long rows, long cols);
+int fitre_layer_norm_backward(fitre_context *ctx, int dtype, int wtype, const void *dy, long lddy,
+                              const void *x, long ldx, const void *gamma, const void *mean,
+                              const void *rstd, void *dx, long lddx, void *dgamma, void *dbeta,
+                              long rows, long cols, real *devPtr);
+
+/* Per row of logits (rows x vocab): logprobs = log p(tokens[row]); lse = log sum exp; entropy of the
+ * row's distribution; and the `top` (0..32) largest entries, topLogprobs / topTokens (rows x top),
+ * ordered by value, the lower index first among equals.  Each output but those of `top` may be
+ * NULL.  A negative token marks a row without one: its log probability is 0.  A token >= vocab gives
+ * NaN.  Entries of -inf have probability zero; a row of nothing else has no distribution: lse and
+ * log probabilities -inf, entropy 0.  A row that holds a NaN or +inf gives NaN (NaN entries rank as -inf among
+ * the alternatives). */
+int fitre_token_logprobs(fitre_context *ctx, int dtype, const void *logits, long ld,
+                         const long long *tokens, long rows, long vocab, void *logprobs, void *lse,
+                         void *entropy, int top, void *topLogprobs, long long *topTokens);
+/* dLogits = dLogprobs * d logprobs / d logits + dEntropy * d entropy / d logits, from the lse (and, with
+ * dEntropy, entropy) of the forward pass.  Either incoming gradient may be NULL.  Rows with a negative token
+ * get the entropy term alone; rows without a distribution get zero; a token >= vocab gives a row of NaN.
+ * dLogits may be logits (same pointer and stride). */
+int fitre_token_logprobs_backward(fitre_context *ctx, int dtype, const void *logits, long ld,
+                                  const long long *tokens, const void *lse, const void *entropy,
+                                  const void *dLogprobs, const void *dEntropy, void *dLogits, long ldd,
+                                  long rows, long vocab);
+
 #ifdef __cplusplus
 }
 #endif
