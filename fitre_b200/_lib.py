@@ -38,6 +38,8 @@ SYMBOLS = [
     "fitre_subsampled_trust_region_kfac", "fitre_write_vector", "fitre_read_vector",
     "fitre_layer_norm_forward", "fitre_layer_norm_backward_mem_required", "fitre_layer_norm_backward",
     "fitre_token_logprobs", "fitre_token_logprobs_backward",
+    "fitre_gated_forward_mem_required", "fitre_gated_forward", "fitre_gated_backward_mem_required",
+    "fitre_gated_backward", "fitre_orthogonalize_mem_required", "fitre_orthogonalize_update", "fitre_synchronize",
 ]
 
 _lib = None
@@ -146,5 +148,12 @@ def load():
     sig("fitre_layer_norm_backward", i, vp, i, i, vp, l, vp, l, vp, vp, vp, vp, l, vp, vp, l, l, vp)
     sig("fitre_token_logprobs", i, vp, i, vp, l, vp, l, l, vp, vp, vp, i, vp, vp)
     sig("fitre_token_logprobs_backward", i, vp, i, vp, l, vp, vp, vp, vp, vp, vp, l, l, l)
+    sig("fitre_gated_forward_mem_required", l, l, l, l)
+    sig("fitre_gated_forward", i, vp, i, i, vp, l, vp, l, vp, l, vp, l, vp, l, vp, l, l, l, l, vp)
+    sig("fitre_gated_backward_mem_required", l, l, l, l)
+    sig("fitre_gated_backward", i, vp, i, i, vp, l, vp, l, vp, l, vp, l, vp, l, vp, l, vp, l, vp, l, vp, l, l, l, l, vp)
+    sig("fitre_orthogonalize_mem_required", l, l, l, l)
+    sig("fitre_orthogonalize_update", i, vp, i, vp, l, l, vp, l, l, l, l, l, i, dbl_p, d, d, vp)
+    sig("fitre_synchronize", i, vp)
     _lib = L
     return L

@@ -64,6 +64,10 @@ class Context:
         if rc != S.OK:
             raise FitreError(rc, self.lib.fitre_last_error(self.h).decode())
 
+    def synchronize(self):
+        """Waits for the stream; raises if a kernel's bounded wait ran out since the last report."""
+        self.check(self.lib.fitre_synchronize(self.h))
+
     @property
     def launches(self):
         return int(self.lib.fitre_launch_count(self.h))
@@ -654,3 +658,81 @@ def tokenLogProbsBackward(ctx, logits, tokens, lse, entropy, dLogprobs, dEntropy
         ctx.h, code, xp, ld, _vector(ctx, tokens, "tokens", rows, torch.int64), _vector(ctx, lse, "lse", rows, stat),
         _vector(ctx, entropy, "entropy", rows, stat), _vector(ctx, dLogprobs, "dLogprobs", rows, stat),
         _vector(ctx, dEntropy, "dEntropy", rows, stat), dp, ldd, rows, vocab))
+
+
+def gatedForwardMemRequired(tokens, width, hidden):
+    """Scratch (doubles) of gatedForward; 0 whenever width is a multiple of 8."""
+    return int(_lib.load().fitre_gated_forward_mem_required(tokens, width, hidden))
+
+
+def gatedForward(ctx, x, wGate, wUp, h, gate=None, up=None, act=S.CNN_ACT_SWISH, devPtr=None):
+    """h = act(x wGate') * (x wUp'); gate / up keep the two products for gatedBackward."""
+    code = _dtype_code(x)
+    xp, ldx = _matrix(ctx, x, "x")
+    tokens, width = x.shape
+    gp, ldwg = _matrix(ctx, wGate, "wGate", None, x.dtype)
+    hidden = wGate.shape[0]
+    if wGate.shape[1] != width:
+        raise FitreError(S.ERR_BAD_ARG, "wGate must have shape (hidden, %d)" % width)
+    up_, ldwu = _matrix(ctx, wUp, "wUp", (hidden, width), x.dtype)
+    hp, ldh = _matrix(ctx, h, "h", (tokens, hidden), x.dtype)
+    g, ldg = _matrix(ctx, gate, "gate", (tokens, hidden), x.dtype) if gate is not None else (None, 0)
+    u, ldu = _matrix(ctx, up, "up", (tokens, hidden), x.dtype) if up is not None else (None, 0)
+    ctx.check(ctx.lib.fitre_gated_forward(
+        ctx.h, code, act, xp, ldx, gp, ldwg, up_, ldwu, hp, ldh, g, ldg, u, ldu, tokens, width, hidden,
+        _scratch(ctx, devPtr, gatedForwardMemRequired(tokens, width, hidden))))
+
+
+def gatedBackwardMemRequired(tokens, width, hidden):
+    """Scratch (doubles) of gatedBackward."""
+    return int(_lib.load().fitre_gated_backward_mem_required(tokens, width, hidden))
+
+
+def gatedBackward(ctx, dh, x, wGate, wUp, gate, up, dx, dwGate, dwUp, act=S.CNN_ACT_SWISH, devPtr=None):
+    """Gradients of gatedForward from dh and the stored gate / up."""
+    code = _dtype_code(x)
+    xp, ldx = _matrix(ctx, x, "x")
+    tokens, width = x.shape
+    gp, ldwg = _matrix(ctx, wGate, "wGate", None, x.dtype)
+    hidden = wGate.shape[0]
+    if wGate.shape[1] != width:
+        raise FitreError(S.ERR_BAD_ARG, "wGate must have shape (hidden, %d)" % width)
+    wide, thin = (hidden, width), (tokens, hidden)
+    up_, ldwu = _matrix(ctx, wUp, "wUp", wide, x.dtype)
+    dhp, lddh = _matrix(ctx, dh, "dh", thin, x.dtype)
+    g, ldg = _matrix(ctx, gate, "gate", thin, x.dtype)
+    u, ldu = _matrix(ctx, up, "up", thin, x.dtype)
+    dxp, lddx = _matrix(ctx, dx, "dx", (tokens, width), x.dtype)
+    dgp, lddwg = _matrix(ctx, dwGate, "dwGate", wide, x.dtype)
+    dup, lddwu = _matrix(ctx, dwUp, "dwUp", wide, x.dtype)
+    ctx.check(ctx.lib.fitre_gated_backward(
+        ctx.h, code, act, dhp, lddh, xp, ldx, gp, ldwg, up_, ldwu, g, ldg, u, ldu, dxp, lddx, dgp, lddwg, dup, lddwu,
+        tokens, width, hidden, _scratch(ctx, devPtr, gatedBackwardMemRequired(tokens, width, hidden))))
+
+
+def orthogonalizeMemRequired(batch, rows, cols):
+    """Scratch (doubles) of orthogonalizeUpdate."""
+    return int(_lib.load().fitre_orthogonalize_mem_required(batch, rows, cols))
+
+
+def orthogonalizeUpdate(ctx, update, out, devPtr, steps=5, coefficients=None, scale=1.0, eps=1e-7):
+    """out (bfloat16) = scale * the Newton-Schulz polynomial of update / (|update|_F + eps): one matrix
+    (rows, cols) or a batch (batch, rows, cols)."""
+    import torch
+    code = _dtype_code(update)
+    if update.dim() not in (2, 3) or tuple(out.shape) != tuple(update.shape):
+        raise FitreError(S.ERR_BAD_ARG, "update and out must be matrices, or batches of matrices, of one shape")
+    if out.dtype != torch.bfloat16:
+        raise FitreError(S.ERR_UNSUPPORTED, "out must be bfloat16")
+    batch = update.shape[0] if update.dim() == 3 else 1
+    if batch == 0:
+        return
+    one, res = (update[0], out[0]) if update.dim() == 3 else (update, out)
+    rows, cols = one.shape
+    ip, ldi = _matrix(ctx, one, "update")
+    op, ldo = _matrix(ctx, res, "out")
+    si, so = (update.stride(0), out.stride(0)) if update.dim() == 3 else (0, 0)
+    coef = (C.c_double * 3)(*coefficients) if coefficients is not None else None
+    ctx.check(ctx.lib.fitre_orthogonalize_update(
+        ctx.h, code, ip, ldi, si, op, ldo, so, batch, rows, cols, int(steps), coef, float(scale), float(eps),
+        _scratch(ctx, devPtr, orthogonalizeMemRequired(batch, rows, cols))))

@@ -11,7 +11,7 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
-SOURCES = ["gemm.cu", "conv_tma.cu", "conv_tf32.cu", "conv_i8.cu", "layers.cu", "peer.cu", "passes.cu", "kfac.cu", "training.cu", "lm_norm.cu", "lm_logprobs.cu", "lm_api.cpp", "model.cpp", "comm.cpp", "cabi.cpp"]
+SOURCES = ["gemm.cu", "conv_tma.cu", "conv_tf32.cu", "conv_i8.cu", "layers.cu", "peer.cu", "passes.cu", "kfac.cu", "training.cu", "lm_norm.cu", "lm_logprobs.cu", "lm_gated.cu", "lm_ortho.cu", "lm_api.cpp", "model.cpp", "comm.cpp", "cabi.cpp"]
 LIB = os.path.join(HERE, "libfitre_b200.so")
 # C++ functions with the reference's own (mangled) names on top of the C ABI
 SHIM_SRC = os.path.join(HERE, "csrc", "reference_shim.cpp")
@@ -26,7 +26,7 @@ def _stale(obj, src):
         return True
     t = os.path.getmtime(obj)
     deps = [src, os.path.join(CSRC, "common.h"), os.path.join(CSRC, "tma_util.cuh"), os.path.join(CSRC, "graphs.h"),
-            os.path.join(CSRC, "lm_common.cuh"),
+            os.path.join(CSRC, "lm_common.cuh"), os.path.join(CSRC, "lm_gemm.cuh"),
             os.path.join(os.path.dirname(HERE), "include", "fitre_b200.h")]
     return any(os.path.getmtime(d) > t for d in deps)
 

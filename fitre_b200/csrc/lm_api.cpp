@@ -73,6 +73,27 @@ void need_token_shape(int dtype, long rows, long vocab) {
                   "token log probabilities: at most 2^28 entries and 2^27 rows");
 }
 
+// Checks the matrices of the gated block; `stored`: g and u are needed.
+void need_gated_shape(int dtype, int act, long tokens, long width, long hidden) {
+    FITRE_REQUIRE(dtype == FITRE_DTYPE_BF16 || dtype == FITRE_DTYPE_F16, FITRE_ERR_UNSUPPORTED,
+                  "gated block: bf16 or fp16 tensors");
+    FITRE_REQUIRE(act == FITRE_CNN_ACT_NONE || act == FITRE_CNN_ACT_SOFTPLUS || act == FITRE_CNN_ACT_RELU ||
+                      act == FITRE_CNN_ACT_SWISH,
+                  FITRE_ERR_UNSUPPORTED, "gated block: activation outside the path");
+    need(tokens >= 0 && width >= 1 && hidden >= 1, "gated block: tokens >= 0, width >= 1 and hidden >= 1");
+    FITRE_REQUIRE(tokens <= (1l << 24) && width <= (1l << 20) && hidden <= (1l << 20), FITRE_ERR_TOO_LARGE,
+                  "gated block: too large");
+}
+// The stride of a matrix of one row never matters; one that TMA takes.
+void settle_stride(long &ld, long rows, long cols) {
+    if (rows <= 1) ld = (cols + 7) / 8 * 8;
+}
+// Operands of the tensor-core products with a width that is a multiple of 8 are read in place.
+void need_readable(const void *p, long ld, long width, const char *what) {
+    FITRE_REQUIRE(width % 8 != 0 || gated_rows_readable(p, ld), FITRE_ERR_UNSUPPORTED,
+                  std::string(what) + ": rows have to start on 16-byte boundaries when the width is a multiple of 8");
+}
+
 }  // namespace
 
 extern "C" {
@@ -177,6 +198,129 @@ int fitre_token_logprobs_backward(fitre_context *ctx, int dtype, const void *log
         a.dlogits = dLogits, a.ldd = ldd;
         token_logprobs_backward(ctx, a);
     });
+}
+
+long fitre_gated_forward_mem_required(long tokens, long width, long hidden) {
+    if (tokens <= 0 || width <= 0 || hidden <= 0 || tokens > (1l << 24) || width > (1l << 20) || hidden > (1l << 20))
+        return 0;
+    return as_doubles(gated_forward_scratch(tokens, width, hidden));
+}
+
+int fitre_gated_forward(fitre_context *ctx, int dtype, int act, const void *x, long ldx, const void *wGate, long ldwg,
+                        const void *wUp, long ldwu, void *h, long ldh, void *gate, long ldg, void *up, long ldu,
+                        long tokens, long width, long hidden, real *devPtr) {
+    return on_context(ctx, [&] {
+        need_gated_shape(dtype, act, tokens, width, hidden);
+        if (tokens == 0) return;
+        need_matrix(x, ldx, tokens, width, dtype, "x");
+        need_matrix(wGate, ldwg, hidden, width, dtype, "wGate");
+        need_matrix(wUp, ldwu, hidden, width, dtype, "wUp");
+        need_matrix(h, ldh, tokens, hidden, dtype, "h");
+        if (gate) need_matrix(gate, ldg, tokens, hidden, dtype, "gate");
+        if (up) need_matrix(up, ldu, tokens, hidden, dtype, "up");
+        settle_stride(ldx, tokens, width), settle_stride(ldwg, hidden, width), settle_stride(ldwu, hidden, width);
+        settle_stride(ldh, tokens, hidden), settle_stride(ldg, tokens, hidden), settle_stride(ldu, tokens, hidden);
+        if (!gated_streams(tokens)) {
+            need_readable(x, ldx, width, "x");
+            need_readable(wGate, ldwg, width, "wGate");
+            need_readable(wUp, ldwu, width, "wUp");
+        }
+        const long scratch = fitre_gated_forward_mem_required(tokens, width, hidden);
+        if (scratch) {
+            need(devPtr && aligned16(devPtr), "gated block: devPtr is NULL or not 16-byte aligned");
+            require_scratch(ctx, scratch, "gated block");
+        }
+        GatedArgs a = {};
+        a.dtype = dtype, a.act = act, a.x = x, a.ldx = ldx, a.wg = wGate, a.ldwg = ldwg, a.wu = wUp, a.ldwu = ldwu;
+        a.h = h, a.ldh = ldh, a.g = gate, a.ldg = ldg, a.u = up, a.ldu = ldu;
+        a.tokens = tokens, a.width = width, a.hidden = hidden, a.scratch = devPtr;
+        gated_forward(ctx, a);
+    });
+}
+
+long fitre_gated_backward_mem_required(long tokens, long width, long hidden) {
+    if (tokens <= 0 || width <= 0 || hidden <= 0 || tokens > (1l << 24) || width > (1l << 20) || hidden > (1l << 20))
+        return 0;
+    return as_doubles(gated_backward_scratch(tokens, width, hidden));
+}
+
+int fitre_gated_backward(fitre_context *ctx, int dtype, int act, const void *dh, long lddh, const void *x, long ldx,
+                         const void *wGate, long ldwg, const void *wUp, long ldwu, const void *gate, long ldg,
+                         const void *up, long ldu, void *dx, long lddx, void *dwGate, long lddwg, void *dwUp,
+                         long lddwu, long tokens, long width, long hidden, real *devPtr) {
+    return on_context(ctx, [&] {
+        need_gated_shape(dtype, act, tokens, width, hidden);
+        need_matrix(dwGate, lddwg, hidden, width, dtype, "dwGate");
+        need_matrix(dwUp, lddwu, hidden, width, dtype, "dwUp");
+        if (tokens == 0) {   // the sum over no tokens
+            const long row = width * dtype_bytes(dtype);
+            FITRE_CUDA(cudaMemset2DAsync(dwGate, (hidden > 1 ? lddwg : width) * dtype_bytes(dtype), 0, row, hidden, ctx->stream));
+            FITRE_CUDA(cudaMemset2DAsync(dwUp, (hidden > 1 ? lddwu : width) * dtype_bytes(dtype), 0, row, hidden, ctx->stream));
+            return;
+        }
+        need_matrix(dh, lddh, tokens, hidden, dtype, "dh");
+        need_matrix(x, ldx, tokens, width, dtype, "x");
+        need_matrix(wGate, ldwg, hidden, width, dtype, "wGate");
+        need_matrix(wUp, ldwu, hidden, width, dtype, "wUp");
+        need_matrix(gate, ldg, tokens, hidden, dtype, "gate");
+        need_matrix(up, ldu, tokens, hidden, dtype, "up");
+        need_matrix(dx, lddx, tokens, width, dtype, "dx");
+        settle_stride(ldx, tokens, width), settle_stride(ldwg, hidden, width), settle_stride(ldwu, hidden, width);
+        settle_stride(lddh, tokens, hidden), settle_stride(ldg, tokens, hidden), settle_stride(ldu, tokens, hidden);
+        settle_stride(lddx, tokens, width), settle_stride(lddwg, hidden, width), settle_stride(lddwu, hidden, width);
+        need_readable(x, ldx, width, "x");
+        need_readable(wGate, ldwg, width, "wGate");
+        need_readable(wUp, ldwu, width, "wUp");
+        need(devPtr && aligned16(devPtr), "gated block backward: devPtr is NULL or not 16-byte aligned");
+        require_scratch(ctx, fitre_gated_backward_mem_required(tokens, width, hidden), "gated block backward");
+        GatedArgs a = {};
+        a.dtype = dtype, a.act = act, a.dh = dh, a.lddh = lddh, a.x = x, a.ldx = ldx, a.wg = wGate, a.ldwg = ldwg;
+        a.wu = wUp, a.ldwu = ldwu, a.g = (void *)gate, a.ldg = ldg, a.u = (void *)up, a.ldu = ldu;
+        a.dx = dx, a.lddx = lddx, a.dwg = dwGate, a.lddwg = lddwg, a.dwu = dwUp, a.lddwu = lddwu;
+        a.tokens = tokens, a.width = width, a.hidden = hidden, a.scratch = devPtr;
+        gated_backward(ctx, a);
+    });
+}
+
+long fitre_orthogonalize_mem_required(long batch, long rows, long cols) {
+    if (batch <= 0 || rows <= 0 || cols <= 0 || batch > 65535 || rows > (1l << 17) || cols > (1l << 17)) return 0;
+    return as_doubles(ortho_scratch(batch, rows, cols));
+}
+
+int fitre_orthogonalize_update(fitre_context *ctx, int dtype, const void *update, long ldu, long strideu, void *out,
+                               long ldo, long strideo, long batch, long rows, long cols, int steps,
+                               const real *coefficients_host, real scale, real eps, real *devPtr) {
+    return on_context(ctx, [&] {
+        need_type(dtype);
+        need(batch >= 0 && rows >= 1 && cols >= 1, "orthogonalised update: batch >= 0, rows >= 1 and cols >= 1");
+        need(steps >= 1 && steps <= 100, "orthogonalised update: 1 to 100 steps");
+        need(std::isfinite(scale) && std::isfinite(eps) && eps >= 0, "orthogonalised update: scale or eps not finite");
+        FITRE_REQUIRE(batch <= 65535 && rows <= (1l << 17) && cols <= (1l << 17), FITRE_ERR_TOO_LARGE,
+                      "orthogonalised update: at most 65535 matrices of 131072 rows and columns");
+        static const real usual[3] = {3.4445, -4.7750, 2.0315};
+        const real *coef = coefficients_host ? coefficients_host : usual;
+        need(std::isfinite(coef[0]) && std::isfinite(coef[1]) && std::isfinite(coef[2]),
+             "orthogonalised update: coefficients not finite");
+        if (batch == 0) return;
+        need_matrix(update, ldu, rows, cols, dtype, "update");
+        need_matrix(out, ldo, rows, cols, FITRE_DTYPE_BF16, "out");
+        const long spanu = rows > 1 ? (rows - 1) * ldu + cols : cols, spano = rows > 1 ? (rows - 1) * ldo + cols : cols;
+        need(batch == 1 || (strideu >= spanu && strideo >= spano), "orthogonalised update: matrices overlap");
+        FITRE_REQUIRE(batch == 1 || (strideu < kMaxElements && strideo < kMaxElements), FITRE_ERR_TOO_LARGE,
+                      "orthogonalised update: spans too many elements");
+        need(devPtr && aligned16(devPtr), "orthogonalised update: devPtr is NULL or not 16-byte aligned");
+        require_scratch(ctx, fitre_orthogonalize_mem_required(batch, rows, cols), "orthogonalised update");
+        OrthoArgs a = {};
+        a.dtype = dtype, a.in = update, a.ldi = ldu, a.istride = batch > 1 ? strideu : 0, a.out = out, a.ldo = ldo;
+        a.ostride = batch > 1 ? strideo : 0, a.batch = batch, a.rows = rows, a.cols = cols, a.steps = steps;
+        for (int i = 0; i < 3; ++i) a.coef[i] = coef[i];
+        a.scale = scale, a.eps = eps, a.scratch = devPtr;
+        orthogonalize(ctx, a);
+    });
+}
+
+int fitre_synchronize(fitre_context *ctx) {
+    return on_context(ctx, [&] { check_device_error(ctx); });
 }
 
 }  // extern "C"

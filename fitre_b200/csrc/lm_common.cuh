@@ -38,6 +38,31 @@ constexpr int kMaxTop = 32;   // alternatives per row: one per lane of a warp
 void token_logprobs(fitre_context *ctx, const LogProbArgs &a);
 void token_logprobs_backward(fitre_context *ctx, const LogProbArgs &a);
 
+struct GatedArgs {
+    int dtype, act;
+    const void *x, *wg, *wu, *dh;
+    void *h, *g, *u;                     // g and u: stored by the forward pass, read by the backward pass
+    void *dx, *dwg, *dwu, *scratch;
+    long ldx, ldwg, ldwu, lddh, ldh, ldg, ldu, lddx, lddwg, lddwu;
+    long tokens, width, hidden;
+};
+void gated_forward(fitre_context *ctx, const GatedArgs &a);
+void gated_backward(fitre_context *ctx, const GatedArgs &a);
+long gated_forward_scratch(long tokens, long width, long hidden);    // bytes
+long gated_backward_scratch(long tokens, long width, long hidden);
+bool gated_rows_readable(const void *p, long ld);
+bool gated_streams(long tokens);   // so few tokens that the forward pass reads its operands in any layout
+
+struct OrthoArgs {
+    int dtype, steps;
+    const void *in;
+    void *out, *scratch;
+    long ldi, istride, ldo, ostride, batch, rows, cols;
+    double coef[3], scale, eps;
+};
+void orthogonalize(fitre_context *ctx, const OrthoArgs &a);
+long ortho_scratch(long batch, long rows, long cols);
+
 constexpr int kLmSms = 148;   // streaming multiprocessors of a B200
 
 namespace {

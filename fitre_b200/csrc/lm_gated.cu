@@ -1,0 +1,294 @@
+// Gated feed-forward block, both projections with the activation and the product in one kernel, and its
+// backward pass.
+//   g = x Wg', u = x Wu', h = act(g) u                         (x: T x D, Wg and Wu: F x D)
+//   dg = dh u act'(g), du = dh act(g);  dx = dg Wg + du Wu,  dWg = dg' x,  dWu = du' x
+// Forward: one product whose B tile holds the gate's rows beside the up projection's, so that the two
+// accumulators of an output element end up in the same thread's registers: act(g) u costs no memory
+// traffic, and the pre-activations are stored only when a backward pass will want them.  Few tokens (a
+// serving loop's single token) are bound by one read of the weights and go to a kernel that streams
+// them past the tokens held in registers.
+// Backward: dg and du are formed once (memory-bound, rounded to the tensors' type because the tensor
+// core takes no wider operand next to 16-bit weights), then dx is one product over both halves of the
+// concatenated inner dimension, and dWg / dWu one launch over both.
+// All sums are fp32; each output is rounded once.
+#include "lm_gemm.cuh"
+
+namespace fitre {
+namespace {
+
+__device__ __forceinline__ float act_value(int act, float g) {
+    switch (act) {
+        case FITRE_CNN_ACT_SWISH: return g / (1.0f + __expf(-g));
+        case FITRE_CNN_ACT_RELU: return fmaxf(g, 0.0f);
+        case FITRE_CNN_ACT_SOFTPLUS: return fmaxf(g, 0.0f) + log1pf(__expf(-fabsf(g)));
+        default: return g;
+    }
+}
+__device__ __forceinline__ float act_slope(int act, float g) {
+    switch (act) {
+        case FITRE_CNN_ACT_SWISH: {
+            const float s = 1.0f / (1.0f + __expf(-g));
+            return s * (1.0f + g * (1.0f - s));
+        }
+        case FITRE_CNN_ACT_RELU: return g > 0.0f ? 1.0f : 0.0f;
+        case FITRE_CNN_ACT_SOFTPLUS: return 1.0f / (1.0f + __expf(-g));
+        default: return 1.0f;
+    }
+}
+
+template <class T>
+struct GatedEpi {
+    struct Params {
+        T *h, *g, *u;
+        long ldh, ldg, ldu;
+        int M, F, act;
+        bool wide;
+    };
+    static constexpr bool kTwoMaps = true;
+    template <int BN>
+    static __device__ __forceinline__ void store(const Params &p, TileAt at, int row, uint32_t tmem) {
+#pragma unroll 1
+        for (int c = 0; c < BN / 2; c += 32) {
+            const int col = at.n * (BN / 2) + c;
+            if (col >= p.F) break;
+            float g[32], u[32];
+            tmem_load32(tmem + c, g);
+            tmem_load32(tmem + BN / 2 + c, u);
+            if (row < p.M) {
+                if (p.g) store_row32(p.g + (long)row * p.ldg, col, p.F, p.wide, g);
+                if (p.u) store_row32(p.u + (long)row * p.ldu, col, p.F, p.wide, u);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) u[i] *= act_value(p.act, g[i]);
+                store_row32(p.h + (long)row * p.ldh, col, p.F, p.wide, u);
+            }
+        }
+    }
+};
+
+// Few tokens: a warp takes one hidden unit at a time and streams its two weight rows.
+constexpr int V_TOKENS = 4, V_THREADS = 256;
+template <class T, int NT, int VEC>
+__global__ void __launch_bounds__(V_THREADS)
+gated_few_kernel(const T *__restrict__ x, long ldx, const T *__restrict__ wg, long ldwg, const T *__restrict__ wu,
+                 long ldwu, T *h, long ldh, T *g_out, long ldg, T *u_out, long ldu, int D, int F, int act) {
+    const int lane = threadIdx.x & 31;
+    for (int f = (blockIdx.x * V_THREADS + threadIdx.x) / 32; f < F; f += gridDim.x * (V_THREADS / 32)) {
+        float g[NT], u[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) g[t] = u[t] = 0.0f;
+        const T *pg = wg + (long)f * ldwg, *pu = wu + (long)f * ldwu;
+#pragma unroll 4
+        for (int d = lane * VEC; d < D; d += 32 * VEC) {
+            const Vec<T, VEC> a = load_vec<T, VEC>(pg + d), b = load_vec<T, VEC>(pu + d);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const Vec<T, VEC> xv = load_vec<T, VEC>(x + t * ldx + d);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float xe = to_acc<float>(xv.v[e]);
+                    g[t] += to_acc<float>(a.v[e]) * xe;
+                    u[t] += to_acc<float>(b.v[e]) * xe;
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                g[t] += __shfl_xor_sync(0xffffffffu, g[t], o);
+                u[t] += __shfl_xor_sync(0xffffffffu, u[t], o);
+            }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            if (lane == t) {
+                if (g_out) g_out[t * ldg + f] = from_acc<T>(g[t]);
+                if (u_out) u_out[t * ldu + f] = from_acc<T>(u[t]);
+                h[t * ldh + f] = from_acc<T>(act_value(act, g[t]) * u[t]);
+            }
+    }
+}
+
+// dg and du, side by side in scratch ([2][T][ld]).
+template <class T, int VEC>
+__global__ void __launch_bounds__(256)
+gated_slopes_kernel(const T *dh, long lddh, const T *g, long ldg, const T *u, long ldu, T *out, long ld, long half,
+                    int F, int act) {
+    const long row = blockIdx.y;
+    const int at = (blockIdx.x * 256 + threadIdx.x) * VEC;
+    if (at >= F) return;
+    const Vec<T, VEC> a = load_vec<T, VEC>(dh + row * lddh + at), b = load_vec<T, VEC>(g + row * ldg + at),
+                      c = load_vec<T, VEC>(u + row * ldu + at);
+    Vec<T, VEC> dg, du;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        const float d = to_acc<float>(a.v[e]), gv = to_acc<float>(b.v[e]);
+        dg.v[e] = from_acc<T>(d * to_acc<float>(c.v[e]) * act_slope(act, gv));
+        du.v[e] = from_acc<T>(d * act_value(act, gv));
+    }
+    store_vec<T, VEC>(out + row * ld + at, dg);
+    store_vec<T, VEC>(out + half + row * ld + at, du);
+}
+
+// A matrix whose rows TMA cannot read, copied to rows that it can.
+template <class T>
+__global__ void __launch_bounds__(256)
+align_rows_kernel(const T *in, long ld, T *out, long ldo, long rows, int cols) {
+    for (long row = blockIdx.x; row < rows; row += gridDim.x)
+        for (int c = threadIdx.x; c < cols; c += 256) out[row * ldo + c] = in[row * ld + c];
+}
+
+long up8(long n) { return (n + 7) / 8 * 8; }
+long up128(long bytes) { return (bytes + 127) / 128 * 128; }
+
+// Scratch that the operands' copies take when `width` is no multiple of 8 (rows that start off the 16-byte grid).
+long staged_bytes(long tokens, long width, long hidden) {
+    if (width % 8 == 0) return 0;
+    return up128(2 * tokens * up8(width)) + 2 * up128(2 * hidden * up8(width));
+}
+
+template <class T>
+struct Operands {
+    const T *x, *wg, *wu;
+    long ldx, ldwg, ldwu;
+};
+// The operands as TMA can read them; `room` (bytes) advances past the copies made.
+template <class T>
+Operands<T> readable(fitre_context *ctx, const GatedArgs &a, char *&room) {
+    Operands<T> o{(const T *)a.x, (const T *)a.wg, (const T *)a.wu, a.ldx, a.ldwg, a.ldwu};
+    if (a.width % 8 == 0) return o;
+    const long ld = up8(a.width);
+    auto copy = [&](const T *in, long ldi, long rows) {
+        T *out = (T *)room;
+        room += up128(2 * rows * ld);
+        align_rows_kernel<T><<<(unsigned)(rows < 16 * kLmSms ? rows : 16 * kLmSms), 256, 0, ctx->stream>>>(
+            in, ldi, out, ld, rows, (int)a.width);
+        check_launch(ctx, "align_rows_kernel");
+        return out;
+    };
+    o.x = copy(o.x, a.ldx, a.tokens);
+    o.wg = copy(o.wg, a.ldwg, a.hidden);
+    o.wu = copy(o.wu, a.ldwu, a.hidden);
+    o.ldx = o.ldwg = o.ldwu = ld;
+    return o;
+}
+
+template <class T> constexpr int fmt_of = sizeof(T) && std::is_same<T, __half>::value ? G_F16 : G_BF16;
+
+template <class T, int CG, int BN>
+void forward_tiles(fitre_context *ctx, const GatedArgs &a, const Operands<T> &o) {
+    GemmArgs<typename GatedEpi<T>::Params> g = {};
+    const int T_ = (int)a.tokens, D = (int)a.width, F = (int)a.hidden;
+    gemm_map(&g.a[0], o.x, D, T_, 1, o.ldx, 0, a_box<CG, BN, false>, fmt_of<T>);
+    gemm_map(&g.b[0], o.wg, D, F, 1, o.ldwg, 0, b_box<CG, BN, false, true>, fmt_of<T>);
+    gemm_map(&g.b[1], o.wu, D, F, 1, o.ldwu, 0, b_box<CG, BN, false, true>, fmt_of<T>);
+    const bool wide = tma_readable(a.h, a.ldh) && (!a.g || tma_readable(a.g, a.ldg)) && (!a.u || tma_readable(a.u, a.ldu));
+    g.epi = {(T *)a.h, (T *)a.g, (T *)a.u, a.ldh, a.ldg, a.ldu, T_, F, a.act, wide};
+    gemm_launch<CG, BN, false, false, GatedEpi<T>>(ctx, g, T_, F, 1, false, D, 1, fmt_of<T>, "gated_tiles_kernel");
+}
+
+// Whether a product has tiles enough for the SM pairs' 256-row tiles; below, 128-row tiles on single SMs
+// keep more of the GPU busy.
+bool pairs_worth(long M, long N, int n_per_tile, int products) {
+    return ((M + 255) / 256) * ((N + n_per_tile - 1) / n_per_tile) * products >= kLmSms / 2;
+}
+
+template <class T, int NT, int VEC>
+void forward_few(fitre_context *ctx, const GatedArgs &a) {
+    const long warps = (a.hidden + 7) / 8;
+    gated_few_kernel<T, NT, VEC><<<(unsigned)(warps < 8 * kLmSms ? warps : 8 * kLmSms), V_THREADS, 0, ctx->stream>>>(
+        (const T *)a.x, a.ldx, (const T *)a.wg, a.ldwg, (const T *)a.wu, a.ldwu, (T *)a.h, a.ldh, (T *)a.g, a.ldg,
+        (T *)a.u, a.ldu, (int)a.width, (int)a.hidden, a.act);
+    check_launch(ctx, "gated_few_kernel");
+}
+template <class T, int VEC>
+void forward_few_as(fitre_context *ctx, const GatedArgs &a) {
+    switch (a.tokens) {
+        case 1: return forward_few<T, 1, VEC>(ctx, a);
+        case 2: return forward_few<T, 2, VEC>(ctx, a);
+        case 3: return forward_few<T, 3, VEC>(ctx, a);
+        default: return forward_few<T, 4, VEC>(ctx, a);
+    }
+}
+
+template <class T>
+void forward_as(fitre_context *ctx, const GatedArgs &a) {
+    if (a.tokens <= V_TOKENS) {
+        const bool wide = a.width % 8 == 0 && tma_readable(a.x, a.ldx) && tma_readable(a.wg, a.ldwg) &&
+                          tma_readable(a.wu, a.ldwu);
+        wide ? forward_few_as<T, 8>(ctx, a) : forward_few_as<T, 1>(ctx, a);
+        return;
+    }
+    char *room = (char *)a.scratch;
+    const Operands<T> o = readable<T>(ctx, a, room);
+    if (pairs_worth(a.tokens, a.hidden, 128, 1)) forward_tiles<T, 2, 256>(ctx, a, o);
+    else forward_tiles<T, 1, 128>(ctx, a, o);
+}
+
+template <class T, int CG, int BN>
+void input_gradient(fitre_context *ctx, const GatedArgs &a, const Operands<T> &o, const T *slopes, long ld, long half) {
+    GemmArgs<typename StoreEpi<T>::Params> g = {};
+    const int T_ = (int)a.tokens, D = (int)a.width, F = (int)a.hidden;
+    gemm_map(&g.a[0], slopes, F, T_, 1, ld, 0, a_box<CG, BN, false>, fmt_of<T>);
+    gemm_map(&g.a[1], slopes + half, F, T_, 1, ld, 0, a_box<CG, BN, false>, fmt_of<T>);
+    gemm_map(&g.b[0], o.wg, D, F, 1, o.ldwg, 0, b_box<CG, BN, true, false>, fmt_of<T>);
+    gemm_map(&g.b[1], o.wu, D, F, 1, o.ldwu, 0, b_box<CG, BN, true, false>, fmt_of<T>);
+    g.epi = {{(T *)a.dx, nullptr}, {a.lddx, 0}, T_, D, tma_readable(a.dx, a.lddx)};
+    gemm_launch<CG, BN, false, true, StoreEpi<T>>(ctx, g, T_, D, 1, false, F, 2, fmt_of<T>, "gated_input_gradient_kernel");
+}
+template <class T, int CG, int BN>
+void weight_gradient(fitre_context *ctx, const GatedArgs &a, const Operands<T> &o, const T *slopes, long ld, long half) {
+    GemmArgs<typename StoreEpi<T>::Params> g = {};
+    const int T_ = (int)a.tokens, D = (int)a.width, F = (int)a.hidden;
+    gemm_map(&g.a[0], slopes, F, T_, 2, ld, half, a_box<CG, BN, true>, fmt_of<T>);
+    gemm_map(&g.b[0], o.x, D, T_, 1, o.ldx, 0, b_box<CG, BN, true, false>, fmt_of<T>);
+    g.g.za = 1;
+    g.epi = {{(T *)a.dwg, (T *)a.dwu}, {a.lddwg, a.lddwu}, F, D,
+             tma_readable(a.dwg, a.lddwg) && tma_readable(a.dwu, a.lddwu)};
+    gemm_launch<CG, BN, true, true, StoreEpi<T>>(ctx, g, F, D, 2, false, T_, 1, fmt_of<T>, "gated_weight_gradient_kernel");
+}
+
+template <class T, int VEC>
+void slopes_as(fitre_context *ctx, const GatedArgs &a, T *slopes, long ld, long half) {
+    const long most = 65535;   // rows a grid's second dimension can count
+    for (long r0 = 0; r0 < a.tokens; r0 += most) {
+        const long n = a.tokens - r0 < most ? a.tokens - r0 : most;
+        gated_slopes_kernel<T, VEC><<<dim3((unsigned)((a.hidden + 256 * VEC - 1) / (256 * VEC)), (unsigned)n), 256, 0,
+                                      ctx->stream>>>(
+            (const T *)a.dh + r0 * a.lddh, a.lddh, (const T *)a.g + r0 * a.ldg, a.ldg, (const T *)a.u + r0 * a.ldu,
+            a.ldu, slopes + r0 * ld, ld, half, (int)a.hidden, a.act);
+        check_launch(ctx, "gated_slopes_kernel");
+    }
+}
+
+template <class T>
+void backward_as(fitre_context *ctx, const GatedArgs &a) {
+    const long ld = up8(a.hidden), half = a.tokens * ld;
+    T *slopes = (T *)a.scratch;
+    char *room = (char *)a.scratch + up128(2 * 2 * half);
+    const bool wide = a.hidden % 8 == 0 && tma_readable(a.dh, a.lddh) && tma_readable(a.g, a.ldg) && tma_readable(a.u, a.ldu);
+    wide ? slopes_as<T, 8>(ctx, a, slopes, ld, half) : slopes_as<T, 1>(ctx, a, slopes, ld, half);
+    const Operands<T> o = readable<T>(ctx, a, room);
+    if (pairs_worth(a.tokens, a.width, 256, 1)) input_gradient<T, 2, 256>(ctx, a, o, slopes, ld, half);
+    else input_gradient<T, 1, 128>(ctx, a, o, slopes, ld, half);
+    if (pairs_worth(a.hidden, a.width, 256, 2)) weight_gradient<T, 2, 256>(ctx, a, o, slopes, ld, half);
+    else weight_gradient<T, 1, 128>(ctx, a, o, slopes, ld, half);
+}
+
+}  // namespace
+
+long gated_forward_scratch(long tokens, long width, long hidden) {
+    return tokens <= V_TOKENS ? 0 : staged_bytes(tokens, width, hidden);
+}
+long gated_backward_scratch(long tokens, long width, long hidden) {
+    return up128(2 * 2 * tokens * up8(hidden)) + staged_bytes(tokens, width, hidden);
+}
+bool gated_streams(long tokens) { return tokens <= V_TOKENS; }
+bool gated_rows_readable(const void *p, long ld) { return tma_readable(p, ld); }
+void gated_forward(fitre_context *ctx, const GatedArgs &a) {
+    a.dtype == FITRE_DTYPE_BF16 ? forward_as<__nv_bfloat16>(ctx, a) : forward_as<__half>(ctx, a);
+}
+void gated_backward(fitre_context *ctx, const GatedArgs &a) {
+    a.dtype == FITRE_DTYPE_BF16 ? backward_as<__nv_bfloat16>(ctx, a) : backward_as<__half>(ctx, a);
+}
+
+}  // namespace fitre

@@ -701,6 +701,45 @@ int fitre_token_logprobs_backward(fitre_context *ctx, int dtype, const void *log
                                   const void *dLogprobs, const void *dEntropy, void *dLogits, long ldd,
                                   long rows, long vocab);
 
+/* Gated feed-forward block: h = act(g) * u with g = x wGate', u = x wUp' (x: tokens x width, weights:
+ * hidden x width, h: tokens x hidden), bf16 or fp16 with fp32 sums.  act: FITRE_CNN_ACT_SWISH, _RELU, _SOFTPLUS
+ * or _NONE.  gate / up (tokens x hidden, may be NULL) receive g and u, which the backward pass reads; h is formed
+ * from their unrounded values.  Up to 4 tokens take any layout; beyond, x, wGate and wUp need rows on 16-byte
+ * boundaries when width is a multiple of 8 (FITRE_ERR_UNSUPPORTED otherwise), and scratch for aligned copies
+ * when it is not: devPtr, fitre_gated_forward_mem_required doubles (0: devPtr may be NULL).  Outputs overlap neither
+ * inputs nor one another. */
+long fitre_gated_forward_mem_required(long tokens, long width, long hidden);
+int fitre_gated_forward(fitre_context *ctx, int dtype, int act, const void *x, long ldx,
+                        const void *wGate, long ldwg, const void *wUp, long ldwu, void *h, long ldh,
+                        void *gate, long ldg, void *up, long ldu, long tokens, long width, long hidden,
+                        real *devPtr);
+/* Its gradients from dh and the stored gate / up: dx = dg wGate + du wUp, dwGate = dg' x, dwUp = du' x with
+ * dg = dh * u * act'(g), du = dh * act(g) rounded to the tensors' type.  Alignment as for the forward pass;
+ * devPtr: fitre_gated_backward_mem_required doubles. */
+long fitre_gated_backward_mem_required(long tokens, long width, long hidden);
+int fitre_gated_backward(fitre_context *ctx, int dtype, int act, const void *dh, long lddh,
+                         const void *x, long ldx, const void *wGate, long ldwg, const void *wUp, long ldwu,
+                         const void *gate, long ldg, const void *up, long ldu, void *dx, long lddx,
+                         void *dwGate, long lddwg, void *dwUp, long lddwu, long tokens, long width,
+                         long hidden, real *devPtr);
+
+/* Orthogonalised update of `batch` equal-sized matrices (rows x cols each, `stride*` elements apart):
+ * X = update / (|update|_F + eps), then `steps` times X <- a X + (b A + c A^2) X with A = X X' (from the smaller
+ * side), out = scale * X in bf16.  coefficients_host: {a, b, c} on the host, NULL = {3.4445, -4.7750, 2.0315}.
+ * The products take fp16 operands scaled by 2^10 and fp32 sums, the iterate itself is held to 22 bits: the
+ * result is within about one bf16 rounding of the exact polynomial as long as the iteration keeps singular
+ * values within about 30 and the coefficients' terms within 60 (it does with the default).  A zero matrix gives zero; one with a NaN or an infinity gives NaN.  out may be update.
+ * devPtr: fitre_orthogonalize_mem_required doubles. */
+long fitre_orthogonalize_mem_required(long batch, long rows, long cols);
+int fitre_orthogonalize_update(fitre_context *ctx, int dtype, const void *update, long ldu, long strideu,
+                               void *out, long ldo, long strideo, long batch, long rows, long cols,
+                               int steps, const real *coefficients_host, real scale, real eps,
+                               real *devPtr);
+
+/* Waits for the context's stream and reports (FITRE_ERR_CUDA) whether a kernel's bounded wait ran out since
+ * the last report: the operators above return before their kernels have run. */
+int fitre_synchronize(fitre_context *ctx);
+
 #ifdef __cplusplus
 }
 #endif
