@@ -26,7 +26,7 @@ def _stale(obj, src):
         return True
     t = os.path.getmtime(obj)
     deps = [src, os.path.join(CSRC, "common.h"), os.path.join(CSRC, "tma_util.cuh"), os.path.join(CSRC, "graphs.h"),
-            os.path.join(CSRC, "lm_common.cuh"), os.path.join(CSRC, "lm_gemm.cuh"),
+            os.path.join(CSRC, "lm_common.cuh"), os.path.join(CSRC, "lm_gemm.cuh"), os.path.join(CSRC, "lm_ring.cuh"), os.path.join(CSRC, "lm_simd.cuh"),
             os.path.join(os.path.dirname(HERE), "include", "fitre_b200.h")]
     return any(os.path.getmtime(d) > t for d in deps)
 

@@ -65,14 +65,14 @@ struct GatedEpi {
     }
 };
 
-// Few tokens: a warp takes one hidden unit at a time and streams its two weight rows.
+// Few tokens: a warp takes one hidden unit and streams its two weight rows.
 constexpr int V_TOKENS = 4, V_THREADS = 256;
 template <class T, int NT, int VEC>
 __global__ void __launch_bounds__(V_THREADS)
 gated_few_kernel(const T *__restrict__ x, long ldx, const T *__restrict__ wg, long ldwg, const T *__restrict__ wu,
                  long ldwu, T *h, long ldh, T *g_out, long ldg, T *u_out, long ldu, int D, int F, int act) {
-    const int lane = threadIdx.x & 31;
-    for (int f = (blockIdx.x * V_THREADS + threadIdx.x) / 32; f < F; f += gridDim.x * (V_THREADS / 32)) {
+    const int lane = threadIdx.x & 31, f = (blockIdx.x * V_THREADS + threadIdx.x) / 32;
+    if (f < F) {
         float g[NT], u[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) g[t] = u[t] = 0.0f;
@@ -194,8 +194,7 @@ bool pairs_worth(long M, long N, int n_per_tile, int products) {
 
 template <class T, int NT, int VEC>
 void forward_few(fitre_context *ctx, const GatedArgs &a) {
-    const long warps = (a.hidden + 7) / 8;
-    gated_few_kernel<T, NT, VEC><<<(unsigned)(warps < 8 * kLmSms ? warps : 8 * kLmSms), V_THREADS, 0, ctx->stream>>>(
+    gated_few_kernel<T, NT, VEC><<<(unsigned)((a.hidden + 7) / 8), V_THREADS, 0, ctx->stream>>>(
         (const T *)a.x, a.ldx, (const T *)a.wg, a.ldwg, (const T *)a.wu, a.ldwu, (T *)a.h, a.ldh, (T *)a.g, a.ldg,
         (T *)a.u, a.ldu, (int)a.width, (int)a.hidden, a.act);
     check_launch(ctx, "gated_few_kernel");

@@ -3,12 +3,17 @@
 //   lse = log sum_j exp x_j,  lp = x_token - lse,  H = lse - sum_j p_j x_j,  p_j = exp(x_j - lse)
 //   dx_j = gl (1[j = token] - p_j) - gH p_j (log p_j + H)
 // Forward: bound by one read of the logits, next to which one exponential per element is all the
-// special-function unit can do, so everything comes out of a single sweep: each thread keeps the running
-// maximum m, s = sum exp(x - m) and t = sum exp(x - m)(x - m) (entropy = log s - t / s, free of the
-// cancellation that large logits would bring), rescaled only when a batch of loads raises its
-// maximum.  The alternatives need no second sweep either: the k-th largest of the threads' maxima is a
-// lower bound of the k-th largest element, so only the few threads whose maximum reaches it have their
-// elements read again (from L2) and filtered into lists that a warp keeps sorted across its lanes.
+// special-function unit can do, so everything comes out of a single sweep: each thread keeps a
+// reference r, s = sum exp(x - r) and t = sum exp(x - r)(x - r) (entropy = log s - t / s, free of the
+// cancellation that large logits would bring).  r follows the running maximum lazily, when a value
+// exceeds it by 10: sums of exponentials up to e^10 lose nothing in fp32, and rescaling becomes rare.
+// The sweep runs on pairs (packed fp32 arithmetic, 16-bit packed maxima): 4.5 instructions per element
+// instead of 8, which would be more than the issue slots one read of memory leaves.  An entry of
+// -inf would put 0 * -inf into t; that is noticed per vector, which is then done again with care.
+// The alternatives need no second sweep either: the k-th largest of the threads' maxima is a
+// lower bound of the k-th largest element, so only the vectors of the few threads whose maximum reaches
+// it are read again (from L2) and filtered into lists that each warp keeps sorted across its lanes; lists
+// are joined by ranking their entries in one another.
 // With few rows a cluster of up to 16 blocks shares a row and joins its statistics and lists over
 // distributed shared memory; no workspace, no atomics, one launch.
 // Backward: one read and one write of the logits, element by element.
@@ -17,6 +22,7 @@
 #include <cfloat>
 
 #include "lm_common.cuh"
+#include "lm_simd.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -73,7 +79,7 @@ template <class A> struct WarpList {
     int k, lane;
     __device__ __forceinline__ WarpList(int k_, int lane_) : k(k_), lane(lane_) {
         e.v = -Num<A>::inf();
-        e.i = 0x7fffffff;
+        e.i = 0x7fffffff;   // none: worse than any entry
     }
     // every lane offers one entry (or none); called by the whole warp
     __device__ __forceinline__ void offer(bool has, A v, int i) {
@@ -102,27 +108,135 @@ template <class A> struct WarpList {
     }
 };
 
-template <class A> __device__ __forceinline__ A warp_max(A v) {
+// The largest value of a warp's lanes.
+__device__ __forceinline__ float warp_max(float v) {
+    // as integers in the same order: one reduction instruction instead of five exchanges
+    const int i = __float_as_int(v);
+    const int k = __reduce_max_sync(0xffffffffu, i ^ ((i >> 31) & 0x7fffffff));
+    return __int_as_float(k ^ ((k >> 31) & 0x7fffffff));
+}
+__device__ __forceinline__ double warp_max(double v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = Num<A>::max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    for (int o = 16; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
 
-constexpr int L_UNROLL = 4;   // 16-byte loads a thread has in flight
+__device__ __forceinline__ float exp2_fast(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// The largest element of a vector; NaN is passed over.
+__device__ __forceinline__ float vec_max(const Vec<__nv_bfloat16, 8> &x) {
+    const __nv_bfloat162 *p = reinterpret_cast<const __nv_bfloat162 *>(x.v);
+    const __nv_bfloat162 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ float vec_max(const Vec<__half, 8> &x) {
+    const __half2 *p = reinterpret_cast<const __half2 *>(x.v);
+    const __half2 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ float vec_max(const Vec<float, 4> &x) {
+    return fmaxf(fmaxf(x.v[0], x.v[1]), fmaxf(x.v[2], x.v[3]));
+}
+__device__ __forceinline__ double vec_max(const Vec<double, 2> &x) { return fmax(x.v[0], x.v[1]); }
+
+constexpr float kLazy = 10.0f;   // how far values may exceed the reference before it follows
+
+// A thread's statistics and its largest element.
+template <class A> struct Running {
+    Stats<A> st{Num<A>::lowest, 0, 0};
+    A top = -Num<A>::inf();
+    // before elements of which `m` is the largest
+    __device__ __forceinline__ void follow(A m) {
+        using N = Num<A>;
+        top = N::max(top, m);
+        if (m - st.m > A(kLazy)) {
+            const A d = N::max_nan(st.m - m, N::floor), c = N::exp_(d);
+            st.t = (st.t + d * st.s) * c;
+            st.s *= c;
+            st.m = m;
+        }
+    }
+    __device__ __forceinline__ void element(A v) {   // with -inf, NaN and overflowing differences
+        using N = Num<A>;
+        const A d = N::max_nan(v - st.m, N::floor), p = N::exp_(d);
+        st.s += p;
+        st.t += p * d;
+    }
+    template <class T, int VEC> __device__ __forceinline__ void vector(const Vec<T, VEC> &x) {
+        if constexpr (sizeof(A) == 8) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) element(to_acc<A>(x.v[e]));
+        } else {
+            using P = Simd<float, 2>;
+            const P back = P::splat(-st.m), l2e = P::splat(1.4426950408889634f);
+            P v[VEC / 2], s = P::splat(0), t = s;
+            widen(x, v);
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) {
+                const P d = add(v[i], back);
+                float a, b;
+                mul(d, l2e).split(a, b);
+                const P p = P::of(exp2_fast(a), exp2_fast(b));
+                s = add(s, p);
+                t = fma(p, d, t);
+            }
+            const float tt = t.sum();
+            if (tt == tt) {
+                st.s += s.sum();
+                st.t += tt;
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) element(to_acc<float>(x.v[e]));
+            }
+        }
+    }
+};
+
+constexpr int kNone = 0x7fffffff;   // place of an entry that is none
+// Joins `count` sorted lists (kMaxTop entries each, a power of two of them) into the first, pairs at a time: the
+// better of a[i] and b[31 - i] are the 32 best of both as a bitonic sequence, which five exchanges sort.
+template <class A> __device__ __forceinline__ void merge_lists(Entry<A> *lists, int count) {
+    const int lane = threadIdx.x & 31;
+    for (int gap = 1; gap < count; gap *= 2) {
+        for (int l = (threadIdx.x >> 5) * 2 * gap; l < count; l += (blockDim.x >> 5) * 2 * gap) {
+            Entry<A> e = lists[l * kMaxTop + lane];
+            const Entry<A> o = lists[(l + gap) * kMaxTop + 31 - lane];
+            if (better(o.v, o.i, e.v, e.i)) e = o;
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) {
+                Entry<A> p;
+                p.v = __shfl_xor_sync(0xffffffffu, e.v, x);
+                p.i = __shfl_xor_sync(0xffffffffu, e.i, x);
+                if (better(p.v, p.i, e.v, e.i) == ((lane & x) == 0)) e = p;
+            }
+            lists[l * kMaxTop + lane] = e;
+        }
+        __syncthreads();
+    }
+}
+
+constexpr int L_UNROLL = 4;      // 16-byte loads a thread has in flight
+constexpr int kMaxParts = 16;    // blocks that may share a row
+constexpr int kRoom = 256;       // candidates a block can rank at once
 
 template <class T, int THREADS, bool TOP>
-__global__ void __launch_bounds__(THREADS, (sizeof(T) == 8 ? 512 : 1024) / THREADS)
+__global__ void __launch_bounds__(THREADS, (sizeof(T) == 8 ? 512 : 768) / THREADS)
 token_logprobs_kernel(const T *__restrict__ logits, long ld, const long long *__restrict__ tokens, int vocab, int top,
                       acc_t<T> *logprobs, acc_t<T> *lse_out, acc_t<T> *entropy, acc_t<T> *top_logprobs,
                       long long *top_tokens) {
     using A = acc_t<T>;
     using N = Num<A>;
     constexpr int VEC = 16 / sizeof(T), WARPS = THREADS / 32;
+    constexpr int LISTS = WARPS > kMaxParts ? WARPS : kMaxParts;
     __shared__ Stats<A> wstat[WARPS];
     __shared__ Stats<A> bstat;                     // this block's part of the row, read by the cluster
-    __shared__ A tmax[TOP ? THREADS : 1];
-    __shared__ A bound_s;
-    __shared__ Entry<A> lists[TOP ? WARPS * kMaxTop : 1], blist[TOP ? kMaxTop : 1];
+    __shared__ A wbound[WARPS];
+    __shared__ int hot[TOP ? THREADS : 1], hots, found;
+    __shared__ Entry<A> room[TOP ? kRoom : 1], lists[TOP ? LISTS * kMaxTop : 1], blist[TOP ? kMaxTop : 1];
     cg::cluster_group cluster = cg::this_cluster();
     const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
     const long row = blockIdx.x / parts;
@@ -137,44 +251,45 @@ token_logprobs_kernel(const T *__restrict__ logits, long ld, const long long *__
     const int edges = head + (hi - tail0);         // fewer than 2 * VEC, at most 14
     const T *xv = x + vbase;
 
-    Stats<A> st{N::lowest, 0, 0};
+    Running<A> run;
+    Vec<T, VEC> raw[L_UNROLL], next[L_UNROLL];
+    int at = tid;
+    // whole batches, the next one's loads issued before this one's arithmetic
+    const int batches = nvec / (THREADS * L_UNROLL);
+    if (batches) {
+#pragma unroll
+        for (int u = 0; u < L_UNROLL; ++u) raw[u] = load_vec<T, VEC>(xv + (long)(at + u * THREADS) * VEC);
+    }
+    for (int b = 0; b < batches; ++b) {
+        at += THREADS * L_UNROLL;
+        if (b + 1 < batches) {
+#pragma unroll
+            for (int u = 0; u < L_UNROLL; ++u) next[u] = load_vec<T, VEC>(xv + (long)(at + u * THREADS) * VEC);
+        }
+        A m = vec_max(raw[0]);
+#pragma unroll
+        for (int u = 1; u < L_UNROLL; ++u) m = N::max(m, vec_max(raw[u]));
+        run.follow(m);
+#pragma unroll
+        for (int u = 0; u < L_UNROLL; ++u) run.vector(raw[u]);
+#pragma unroll
+        for (int u = 0; u < L_UNROLL; ++u) raw[u] = next[u];
+    }
+#pragma unroll
+    for (int u = 0; u < L_UNROLL; ++u)
+        if (at + u * THREADS < nvec) raw[u] = load_vec<T, VEC>(xv + (long)(at + u * THREADS) * VEC);
+#pragma unroll
+    for (int u = 0; u < L_UNROLL; ++u)
+        if (at + u * THREADS < nvec) {
+            run.follow(vec_max(raw[u]));
+            run.vector(raw[u]);
+        }
     if (tid < edges) {
-        const int at = tid < head ? lo + tid : tail0 + (tid - head);
-        const A v = to_acc<A>(x[at]);
-        st.m = N::max(st.m, v);
-        const A d = N::max_nan(v - st.m, N::floor);
-        st.s = N::exp_(d);
-        st.t = st.s * d;
+        const A v = to_acc<A>(x[tid < head ? lo + tid : tail0 + (tid - head)]);
+        run.follow(v);
+        run.element(v);
     }
-    for (int at = tid; at < nvec; at += THREADS * L_UNROLL) {
-        Vec<T, VEC> raw[L_UNROLL];
-#pragma unroll
-        for (int u = 0; u < L_UNROLL; ++u)
-            if (at + u * THREADS < nvec) raw[u] = load_vec<T, VEC>(xv + (long)(at + u * THREADS) * VEC);
-#pragma unroll
-        for (int u = 0; u < L_UNROLL; ++u)
-            if (at + u * THREADS < nvec) {
-                A v[VEC], m = st.m;
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    v[e] = to_acc<A>(raw[u].v[e]);
-                    m = N::max(m, v[e]);
-                }
-                if (m > st.m) {
-                    const A d = N::max_nan(st.m - m, N::floor), c = N::exp_(d);
-                    st.t = (st.t + d * st.s) * c;
-                    st.s *= c;
-                    st.m = m;
-                }
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const A d = N::max_nan(v[e] - st.m, N::floor), p = N::exp_(d);
-                    st.s += p;
-                    st.t += p * d;
-                }
-            }
-    }
-    const A mine = st.m > N::lowest ? st.m : -N::inf();   // a lower bound of this thread's maximum
+    Stats<A> st = run.st;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         Stats<A> other;
@@ -184,115 +299,121 @@ token_logprobs_kernel(const T *__restrict__ logits, long ld, const long long *__
         st = (lane & o) ? join(other, st) : join(st, other);
     }
     if (lane == 0) wstat[warp] = st;
-    if (TOP) tmax[tid] = mine;
+    if (TOP) {
+        // the q-th largest of each warp's maxima, q = top / WARPS rounded up: the smallest of these has at least
+        // `top` elements at or above it
+        A best = run.top, b = best;
+        for (int q = 0; q < (top + WARPS - 1) / WARPS; ++q) {
+            b = warp_max(best);
+            const unsigned who = __ballot_sync(0xffffffffu, best == b);
+            if (lane == __ffs(who) - 1) best = -N::inf();
+        }
+        if (lane == 0) wbound[warp] = b;
+        if (tid == 0) hots = found = 0;
+        if (tid < kMaxTop) blist[tid] = Entry<A>{-N::inf(), kNone};
+    }
     __syncthreads();
     if (tid == 0) {
         Stats<A> r = wstat[0];
+#pragma unroll
         for (int w = 1; w < WARPS; ++w) r = join(r, wstat[w]);
         bstat = r;
     }
     if (TOP) {
-        if (warp == WARPS - 1) {
-            // the top-th largest of the threads' maxima, by taking the maximum out `top` times
-            A v[WARPS];
+        A bound = wbound[0];
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) v[w] = tmax[w * 32 + lane];
-            A b = -N::inf();
-            for (int r = 0; r < top; ++r) {
-                A best = v[0];
+        for (int w = 1; w < WARPS; ++w) bound = bound < wbound[w] ? bound : wbound[w];
+        if (run.top >= bound) hot[atomicAdd(&hots, 1)] = tid;   // any order: entries are ranked by value and place
+        const bool edge = tid < edges;
+        const int edge_at = tid < head ? lo + tid : tail0 + (tid - head);
+        A edge_v = edge ? to_acc<A>(x[edge_at]) : -N::inf();
+        if (edge_v != edge_v) edge_v = -N::inf();               // a NaN ranks as -inf
+        if (edge && edge_v >= bound) room[atomicAdd(&found, 1)] = Entry<A>{edge_v, edge_at};
+        __syncthreads();
+        // vectors of the hot threads, in rising order of place
+        const int rounds = (nvec + THREADS - 1) / THREADS, hotn = hots;
+        auto each = [&](auto &&use) {
+            for (int i0 = warp * 32; i0 < rounds * hotn; i0 += THREADS) {
+                const int i = i0 + lane, j = i / hotn;
+                const int vec = j < rounds ? hot[i - j * hotn] + j * THREADS : nvec;
+                const bool in = vec < nvec;
+                Vec<T, VEC> raw;
+                if (in) raw = load_vec<T, VEC>(xv + (long)vec * VEC);
 #pragma unroll
-                for (int w = 1; w < WARPS; ++w) best = N::max(best, v[w]);
-                b = warp_max(best);
-                const unsigned who = __ballot_sync(0xffffffffu, best == b);
-                if (lane == __ffs(who) - 1) {
-                    bool out = false;
-#pragma unroll
-                    for (int w = 0; w < WARPS; ++w)
-                        if (!out && v[w] == b) {
-                            v[w] = -N::inf();
-                            out = true;
-                        }
+                for (int e = 0; e < VEC; ++e) {
+                    A v = in ? to_acc<A>(raw.v[e]) : -N::inf();
+                    if (v != v) v = -N::inf();
+                    use(in && v >= bound, v, vbase + vec * VEC + e);
                 }
             }
-            if (lane == 0) bound_s = b;
-        }
-        __syncthreads();
-        const A bound = bound_s;
-        WarpList<A> list(top, lane);
-        if (warp == 0) {
-            const bool has = lane < edges;
-            const int at = lane < head ? lo + lane : tail0 + (lane - head);
-            A v = has ? to_acc<A>(x[at]) : -N::inf();
-            if (v != v) v = -N::inf();             // a NaN ranks as -inf
-            list.offer(has && v >= bound, v, at);
-        }
-        int turn = 0;
-        for (int w = 0; w < WARPS; ++w) {
-            // threads of warp w whose maximum reaches the bound, dealt out to the warps
-            unsigned hot = __ballot_sync(0xffffffffu, tmax[w * 32 + lane] >= bound);
-            for (; hot; hot &= hot - 1) {
-                if (turn++ % WARPS != warp) continue;
-                const int owner = w * 32 + __ffs(hot) - 1;
-                for (int j0 = 0; owner + j0 * THREADS < nvec; j0 += 32) {
-                    const int at = owner + (j0 + lane) * THREADS;
-                    const bool in = at < nvec;
-                    Vec<T, VEC> raw;
-                    if (in) raw = load_vec<T, VEC>(xv + (long)at * VEC);
-                    A v[VEC];
-                    bool any = false;
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        v[e] = in ? to_acc<A>(raw.v[e]) : -N::inf();
-                        if (v[e] != v[e]) v[e] = -N::inf();
-                        any = any || (in && v[e] >= bound);
-                    }
-                    if (__any_sync(0xffffffffu, any)) {
-#pragma unroll
-                        for (int e = 0; e < VEC; ++e) list.offer(in && v[e] >= bound, v[e], vbase + at * VEC + e);
-                    }
-                }
+        };
+        each([&](bool has, A v, int i) {
+            if (has) {
+                const int at = atomicAdd(&found, 1);
+                if (at < kRoom) room[at] = Entry<A>{v, i};
             }
-        }
-        if (lane < top) lists[warp * kMaxTop + lane] = list.e;
+        });
         __syncthreads();
-        if (warp == 0) {
-            for (int w = 1; w < WARPS; ++w) {
-                const Entry<A> o = lists[w * kMaxTop + lane];
-                list.offer(lane < top && o.i != 0x7fffffff, o.v, o.i);
+        if (found <= kRoom) {
+            for (int i = tid; i < found; i += THREADS) {
+                const Entry<A> e = room[i];
+                int rank = 0;
+                for (int o = 0; o < found; ++o) rank += better(room[o].v, room[o].i, e.v, e.i) ? 1 : 0;
+                if (rank < top) blist[rank] = e;
             }
-            if (lane < top) blist[lane] = list.e;
+        } else {
+            // too many equal values: sorted lists, in which a later equal value displaces nothing
+            WarpList<A> list(top, lane);
+            if (warp == 0) list.offer(edge && edge_v >= bound, edge_v, edge_at);
+            each([&](bool has, A v, int i) { list.offer(has, v, i); });
+            lists[warp * kMaxTop + lane] = lane < top ? list.e : Entry<A>{-N::inf(), kNone};
+            __syncthreads();
+            merge_lists(lists, WARPS);
+            if (tid < top) blist[tid] = lists[tid];
         }
     }
     if (parts > 1) cluster.sync();
     else __syncthreads();
-    if (part == 0 && warp == 0) {
-        Stats<A> r = bstat;
-        for (int p = 1; p < parts; ++p) r = join(r, *cluster.map_shared_rank(&bstat, p));
-        const bool none = r.s == A(0);             // every logit is -inf: no distribution
-        const A logs = N::log_(r.s);
-        const A lse = none ? -N::inf() : r.m + logs;
-        if (lane == 0) {
-            if (lse_out) lse_out[row] = lse;
-            if (entropy) entropy[row] = none ? A(0) : logs - r.t / r.s;
-            if (logprobs) {
-                const long long tok = tokens[row];
-                A lp = 0;
-                if (tok >= vocab) lp = N::inf() - N::inf();
-                else if (tok >= 0) lp = none ? -N::inf() : (to_acc<A>(x[tok]) - r.m) - logs;
-                logprobs[row] = lp;
-            }
+    if (part == 0) {
+        const Entry<A> *final_list = blist;
+        if (TOP && parts > 1) {
+            for (int i = tid; i < parts * kMaxTop; i += THREADS)
+                lists[i] = cluster.map_shared_rank(blist, i / kMaxTop)[i % kMaxTop];
+            __syncthreads();
+            merge_lists(lists, parts);
+            final_list = lists;
         }
-        if (TOP) {
-            WarpList<A> list(top, lane);
-            if (lane < top) list.e = blist[lane];
-            for (int p = 1; p < parts; ++p) {
-                Entry<A> o{-N::inf(), 0x7fffffff};
-                if (lane < top) o = cluster.map_shared_rank(blist, p)[lane];
-                list.offer(o.i != 0x7fffffff, o.v, o.i);
+        if (warp == 0) {
+            Stats<A> r{N::lowest, 0, 0};
+            if (lane < parts) r = *cluster.map_shared_rank(&bstat, lane);
+#pragma unroll
+            for (int o = kMaxParts / 2; o > 0; o >>= 1) {
+                Stats<A> other;
+                other.m = __shfl_xor_sync(0xffffffffu, r.m, o);
+                other.s = __shfl_xor_sync(0xffffffffu, r.s, o);
+                other.t = __shfl_xor_sync(0xffffffffu, r.t, o);
+                r = (lane & o) ? join(other, r) : join(r, other);
             }
-            if (lane < top) {
-                top_tokens[row * top + lane] = list.e.i;
-                top_logprobs[row * top + lane] = none ? -N::inf() : (list.e.v - r.m) - logs;
+            r.m = __shfl_sync(0xffffffffu, r.m, 0);
+            r.s = __shfl_sync(0xffffffffu, r.s, 0);
+            r.t = __shfl_sync(0xffffffffu, r.t, 0);
+            const bool none = r.s == A(0);         // every logit is -inf: no distribution
+            const A logs = N::log_(r.s);
+            if (lane == 0) {
+                if (lse_out) lse_out[row] = none ? -N::inf() : r.m + logs;
+                if (entropy) entropy[row] = none ? A(0) : logs - r.t / r.s;
+                if (logprobs) {
+                    const long long tok = tokens[row];
+                    A lp = 0;
+                    if (tok >= vocab) lp = N::inf() - N::inf();
+                    else if (tok >= 0) lp = none ? -N::inf() : (to_acc<A>(x[tok]) - r.m) - logs;
+                    logprobs[row] = lp;
+                }
+            }
+            if (TOP && lane < top) {
+                const Entry<A> e = final_list[lane];
+                top_tokens[row * top + lane] = e.i;
+                top_logprobs[row * top + lane] = none ? -N::inf() : (e.v - r.m) - logs;
             }
         }
     }
@@ -313,6 +434,16 @@ token_logprobs_backward_kernel(const T *logits, long ld, const long long *__rest
     const int chunk = (int)(blockIdx.x - row * chunks), tid = threadIdx.x;
     const T *x = logits + row * ld;
     T *dx = dlogits + row * ldd;
+    int head = VEC > 1 ? (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T) : 0;
+    head = head < vocab ? head : vocab;
+    const int nvec = (vocab - head) / VEC, tail0 = head + nvec * VEC, edges = head + (vocab - tail0);
+    // the row's vectors in equal shares, none above THREADS * B_UNROLL
+    const int share = (nvec + chunks - 1) / chunks, v0 = chunk * share + tid;
+    const int vend = chunk * share + share < nvec ? chunk * share + share : nvec;
+    Vec<T, VEC> raw[B_UNROLL];
+#pragma unroll
+    for (int u = 0; u < B_UNROLL; ++u)
+        if (v0 + u * THREADS < vend) raw[u] = load_vec<T, VEC>(x + head + (long)(v0 + u * THREADS) * VEC);
     const A z = lse[row];
     const bool none = z == -N::inf();
     const long long tok = dlogprobs ? tokens[row] : -1;
@@ -320,32 +451,47 @@ token_logprobs_backward_kernel(const T *logits, long ld, const long long *__rest
     if (tok >= vocab) gl = N::inf() - N::inf();
     const A gh = dentropy ? dentropy[row] : A(0), h = dentropy ? entropy[row] : A(0);
     const int hot = tok >= 0 && tok < vocab ? (int)tok : -1;
+    // an element with care for -inf, NaN and the given token
     auto one = [&](A v, int at) {
         const A lp = N::max_nan(v - z, N::floor), p = N::exp_(lp);
         A g = -p * (gl + gh * (lp + h));
-        if (p == A(0)) g = gl != gl ? gl : A(0);   // nothing times an overflowing logarithm is nothing
+        if (p == A(0)) g = gl + gh != gl + gh ? gl + gh : A(0);   // nothing times an overflowing logarithm is nothing
         if (at == hot) g += gl;
         return none ? A(0) : g;
     };
-    int head = VEC > 1 ? (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T) : 0;
-    head = head < vocab ? head : vocab;
-    const int nvec = (vocab - head) / VEC, tail0 = head + nvec * VEC, edges = head + (vocab - tail0);
     if (chunk == 0 && tid < edges) {
         const int at = tid < head ? tid : tail0 + (tid - head);
         dx[at] = from_acc<T>(one(to_acc<A>(x[at]), at));
     }
-    const int v0 = chunk * THREADS * B_UNROLL + tid;
-    Vec<T, VEC> raw[B_UNROLL];
 #pragma unroll
     for (int u = 0; u < B_UNROLL; ++u)
-        if (v0 + u * THREADS < nvec) raw[u] = load_vec<T, VEC>(x + head + (long)(v0 + u * THREADS) * VEC);
-#pragma unroll
-    for (int u = 0; u < B_UNROLL; ++u)
-        if (v0 + u * THREADS < nvec) {
+        if (v0 + u * THREADS < vend) {
             const int at = head + (v0 + u * THREADS) * VEC;
             Vec<T, VEC> o;
+            bool careful = true;
+            if constexpr (VEC > 1 && sizeof(A) == 4) {
+                // pairs: -p (gl + gh (lp + h)) = p (c0 + c1 lp); a sum of the results tells whether one is no number
+                using P = Simd<float, 2>;
+                const P back = P::splat(-z), l2e = P::splat(1.4426950408889634f), c0 = P::splat(-(gl + gh * h)),
+                        c1 = P::splat(-gh);
+                P v[VEC / 2], seen = P::splat(0);
+                widen(raw[u], v);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) o.v[e] = from_acc<T>(one(to_acc<A>(raw[u].v[e]), at + e));
+                for (int i = 0; i < VEC / 2; ++i) {
+                    const P lp = add(v[i], back);
+                    float a, b;
+                    mul(lp, l2e).split(a, b);
+                    v[i] = mul(P::of(exp2_fast(a), exp2_fast(b)), fma(c1, lp, c0));
+                    seen = add(seen, v[i]);
+                }
+                const float all = seen.sum();
+                careful = all != all || (unsigned)(hot - at) < (unsigned)VEC;
+                o = narrowed<T, VEC>(v);
+            }
+            if (careful) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) o.v[e] = from_acc<T>(one(to_acc<A>(raw[u].v[e]), at + e));
+            }
             store_vec<T, VEC>(dx + at, o);
         }
 }
@@ -379,7 +525,7 @@ void launch_logprobs(fitre_context *ctx, const LogProbArgs &a, int parts) {
 // Blocks that share a row: more while the rows alone leave SMs idle, but no slice under 4096 logits.
 int parts_for(long rows, int vocab) {
     int parts = 1;
-    while (parts < 16 && rows * parts < kLmSms && vocab / (2 * parts) >= 4096) parts *= 2;
+    while (parts < kMaxParts && rows * parts < kLmSms && vocab / (2 * parts) >= 4096) parts *= 2;
     return parts;
 }
 

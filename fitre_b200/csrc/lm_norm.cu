@@ -5,13 +5,18 @@
 // Both passes are bound by HBM, so each element is read once: a row lives in the registers of the G
 // threads that share it (16 elements each, 32 to 1024 threads per row chosen by the row's length),
 // the mean is subtracted before squaring (two reductions over registers cost nothing next to
-// memory), and the following row's loads are issued before this row's reductions wait.  gamma and
-// beta are re-read per row: after the first row they come from the SM's L1.  Rows longer than
-// 16 x 1024 elements go through a form that re-reads the row (from L2) per pass.
+// memory).  gamma and beta are re-read per row: after the first row they come from the SM's L1.
+//   * forward, up to 1024 elements: a warp per row, no barrier;
+//   * wider rows on 16-byte boundaries: blocks that stay resident and have their next rows copied into a
+//     ring in shared memory by bulk copies, which keep more bytes in flight than registers could;
+//   * other rows: the same blocks with element-wise loads into registers, one row ahead;
+//   * rows longer than 16 x 1024 elements: a form that re-reads the row (from L2) per pass.
 // The weight gradient is summed in a fixed order without atomics: every block keeps the column sums of
 // its rows in registers, writes one row of partial sums, and a second kernel adds those rows.
 // Sums, mean and reciprocal deviation are fp32 (fp64 for fp64 tensors).
 #include "lm_common.cuh"
+#include "lm_ring.cuh"
+#include "lm_simd.cuh"
 
 namespace fitre {
 namespace {
@@ -46,84 +51,210 @@ __device__ __forceinline__ void group_sum2(A &a, A &b, A *buf, int &slot) {
     }
 }
 
+template <int G, class A>
+__device__ __forceinline__ A group_sum(A a, A *buf, int &slot) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    if (G > 32) {
+        constexpr int W = G / 32;
+        A *s = buf + slot * 2 * W;
+        slot ^= 1;
+        if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = a;
+        __syncthreads();
+        a = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) a += s[w];
+    }
+    return a;
+}
+
 template <int G> constexpr int norm_threads = G > 32 ? G : 256;   // threads of a block
 template <class A> __device__ __forceinline__ A rsqrt_acc(A v);
 template <> __device__ __forceinline__ float rsqrt_acc<float>(float v) { return 1.0f / sqrtf(v); }
 template <> __device__ __forceinline__ double rsqrt_acc<double>(double v) { return 1.0 / sqrt(v); }
 
+
+// The row's elements that one thread of a group holds: chunks c of VEC consecutive elements at (c G + t) VEC,
+// as packs of accumulators.
+template <class T, int VEC, int G, int CH> struct RowPart {
+    using A = acc_t<T>;
+    using P = SimdOf<T, VEC>;
+    static constexpr int PV = VEC / kPack<VEC>;   // packs in a chunk
+    P v[CH][PV];
+    int left;                                     // chunk c exists while c * G * VEC < left
+    __device__ __forceinline__ RowPart(int cols, int t) : left(cols - t * VEC) {}
+    __device__ __forceinline__ bool has(int c) const { return c * G * VEC < left; }
+    __device__ __forceinline__ void set(int c, const Vec<T, VEC> &x) { widen(x, v[c]); }
+    __device__ __forceinline__ void clear(int c) {
+#pragma unroll
+        for (int i = 0; i < PV; ++i) v[c][i] = P::splat(A(0));
+    }
+    __device__ __forceinline__ A sum() const {
+        P s = P::splat(A(0));
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < PV; ++i) s = add(s, v[c][i]);
+        return s.sum();
+    }
+    // subtracts the mean; returns the sum of the squares that remain
+    __device__ __forceinline__ A centre(A m) {
+        const P back = P::splat(-m);
+        P q = P::splat(A(0));
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+            if (has(c)) {
+#pragma unroll
+                for (int i = 0; i < PV; ++i) {
+                    v[c][i] = add(v[c][i], back);
+                    q = fma(v[c][i], v[c][i], q);
+                }
+            }
+        return q.sum();
+    }
+    // y = v r gamma + beta, `gamma`, `beta` and `y` at this thread's first element
+    template <class W> __device__ __forceinline__ void store(A r, const W *gamma, const W *beta, T *y) const {
+        const P scale = P::splat(r);
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+            if (has(c)) {
+                P o[PV], w[PV];
+#pragma unroll
+                for (int i = 0; i < PV; ++i) o[i] = mul(v[c][i], scale);
+                if (gamma) {
+                    widen(load_vec<W, VEC>(gamma + c * G * VEC), w);
+#pragma unroll
+                    for (int i = 0; i < PV; ++i) o[i] = mul(o[i], w[i]);
+                }
+                if (beta) {
+                    widen(load_vec<W, VEC>(beta + c * G * VEC), w);
+#pragma unroll
+                    for (int i = 0; i < PV; ++i) o[i] = add(o[i], w[i]);
+                }
+                store_vec<T, VEC>(y + c * G * VEC, narrowed<T, VEC>(o));
+            }
+    }
+};
+
+// Blocks that stay resident, G threads per row, the next row's elements loaded one row ahead.
 template <class T, class W, int VEC, int G>
-__global__ void __launch_bounds__(norm_threads<G>, (sizeof(T) == 8 ? 512 : 1024) / norm_threads<G> > 0
-                                                         ? (sizeof(T) == 8 ? 512 : 1024) / norm_threads<G>
-                                                         : 1)
+__global__ void __launch_bounds__(G, (sizeof(T) == 8 ? 512 : 1024) / G > 0 ? (sizeof(T) == 8 ? 512 : 1024) / G : 1)
 layer_norm_kernel(const T *x, long ldx, const W *__restrict__ gamma, const W *__restrict__ beta, T *y, long ldy,
                   acc_t<T> *mean, acc_t<T> *rstd, long rows, int cols, double eps) {
     using A = acc_t<T>;
     constexpr int CH = N_ELEMS / VEC;
-    constexpr int RPB = norm_threads<G> / G;   // rows a block works on at a time
-    __shared__ A buf[G > 32 ? 4 * (G / 32) : 1];
-    const int t = threadIdx.x % G;
-    const long step = (long)gridDim.x * RPB;
-    long row = (long)blockIdx.x * RPB + threadIdx.x / G;
+    __shared__ A buf[4 * (G / 32)];
+    const int t = threadIdx.x;
     int slot = 0;
+    x += t * VEC;
+    y += t * VEC;
+    if (gamma) gamma += t * VEC;
+    if (beta) beta += t * VEC;
+    RowPart<T, VEC, G, CH> part(cols, t);
     Vec<T, VEC> next[CH];
-    if (row < rows) {
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
-            if ((c * G + t) * VEC < cols) next[c] = load_vec<T, VEC>(x + row * ldx + (c * G + t) * VEC);
-    }
-    for (; row < rows; row += step) {
-        A v[N_ELEMS];
+    for (int c = 0; c < CH; ++c)
+        if (part.has(c)) next[c] = load_vec<T, VEC>(x + blockIdx.x * ldx + c * G * VEC);
+    for (long row = blockIdx.x; row < rows; row += gridDim.x) {
+        const long after = row + gridDim.x;
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e)
-                v[c * VEC + e] = (c * G + t) * VEC < cols ? to_acc<A>(next[c].v[e]) : A(0);
-        if (row + step < rows) {
+        for (int c = 0; c < CH; ++c) {
+            if (part.has(c)) part.set(c, next[c]);
+            else part.clear(c);
+        }
+        if (after < rows) {
 #pragma unroll
             for (int c = 0; c < CH; ++c)
-                if ((c * G + t) * VEC < cols) next[c] = load_vec<T, VEC>(x + (row + step) * ldx + (c * G + t) * VEC);
+                if (part.has(c)) next[c] = load_vec<T, VEC>(x + after * ldx + c * G * VEC);
         }
-        A s = 0, unused = 0;
-#pragma unroll
-        for (int i = 0; i < N_ELEMS; ++i) s += v[i];
-        group_sum2<G>(s, unused, buf, slot);
-        const A m = s / (A)cols;
-        A q = 0;
-        unused = 0;
-#pragma unroll
-        for (int c = 0; c < CH; ++c)
-            if ((c * G + t) * VEC < cols) {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const A d = v[c * VEC + e] - m;
-                    v[c * VEC + e] = d;
-                    q += d * d;
-                }
-            }
-        group_sum2<G>(q, unused, buf, slot);
-        const A r = rsqrt_acc<A>(q / (A)cols + (A)eps);
+        const A m = group_sum<G>(part.sum(), buf, slot) / (A)cols;
+        const A r = rsqrt_acc<A>(group_sum<G>(part.centre(m), buf, slot) / (A)cols + (A)eps);
         if (t == 0) {
             if (mean) mean[row] = m;
             if (rstd) rstd[row] = r;
         }
+        part.store(r, gamma, beta, y + row * ldy);
+    }
+}
+
+// A warp per row of up to 1024 elements, 32 to a lane.
+constexpr int N_WIDE = 32;
+template <class T, class W, int VEC>
+__global__ void __launch_bounds__(256, sizeof(T) == 8 ? 2 : 4)
+layer_norm_warp_kernel(const T *x, long ldx, const W *__restrict__ gamma, const W *__restrict__ beta, T *y, long ldy,
+                       acc_t<T> *mean, acc_t<T> *rstd, long rows, int cols, double eps) {
+    using A = acc_t<T>;
+    constexpr int CH = N_WIDE / VEC;
+    const int t = threadIdx.x & 31;
+    const long row = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    x += row * ldx + t * VEC;
+    RowPart<T, VEC, 32, CH> part(cols, t);
+    int slot = 0;
+    {
+        Vec<T, VEC> raw[CH];
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+            if (part.has(c)) raw[c] = load_vec<T, VEC>(x + c * 32 * VEC);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const int at = (c * G + t) * VEC;
-            if (at < cols) {
-                Vec<T, VEC> o;
-                Vec<W, VEC> g, b;
-                if (gamma) g = load_vec<W, VEC>(gamma + at);
-                if (beta) b = load_vec<W, VEC>(beta + at);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    A w = v[c * VEC + e] * r;
-                    if (gamma) w *= to_acc<A>(g.v[e]);
-                    if (beta) w += to_acc<A>(b.v[e]);
-                    o.v[e] = from_acc<T>(w);
-                }
-                store_vec<T, VEC>(y + row * ldy + at, o);
-            }
+            if (part.has(c)) part.set(c, raw[c]);
+            else part.clear(c);
         }
+    }
+    const A m = group_sum<32>(part.sum(), (A *)nullptr, slot) / (A)cols;
+    const A r = rsqrt_acc<A>(group_sum<32>(part.centre(m), (A *)nullptr, slot) / (A)cols + (A)eps);
+    if (t == 0) {
+        if (mean) mean[row] = m;
+        if (rstd) rstd[row] = r;
+    }
+    part.store(r, gamma ? gamma + t * VEC : gamma, beta ? beta + t * VEC : beta, y + row * ldy + t * VEC);
+}
+
+// Rows on 16-byte boundaries through a ring of `stages` rows in shared memory.
+template <class T, class W, int VEC, int G>
+__global__ void __launch_bounds__(G, 1024 / G)
+layer_norm_ring_kernel(const T *x, long ldx, const W *__restrict__ gamma, const W *__restrict__ beta, T *y, long ldy,
+                       acc_t<T> *mean, acc_t<T> *rstd, long rows, int cols, double eps, int stages, int *err) {
+    using A = acc_t<T>;
+    constexpr int CH = N_ELEMS / VEC;
+    extern __shared__ __align__(16) unsigned char ring_raw[];
+    __shared__ unsigned long long bars[kRingMax];
+    __shared__ A buf[4 * (G / 32)];
+    const int t = threadIdx.x;
+    const long step = gridDim.x;
+    int slot = 0;
+    RowRing ring(ring_raw, bars, stages, cols * (int)sizeof(T));
+    ring.init();
+    if (t == 0)
+        for (int i = 0; i < stages; ++i)
+            if (blockIdx.x + i * step < rows) ring.fill(i, x + (blockIdx.x + i * step) * ldx);
+    y += t * VEC;
+    if (gamma) gamma += t * VEC;
+    if (beta) beta += t * VEC;
+    RowPart<T, VEC, G, CH> part(cols, t);
+    for (long row = blockIdx.x; row < rows; row += step) {
+        if (!ring.wait()) {
+            if (t == 0) atomicExch(err, 1);
+            return;
+        }
+        const T *in = (const T *)ring.data() + t * VEC;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            if (part.has(c)) part.set(c, load_vec<T, VEC>(in + c * G * VEC));
+            else part.clear(c);
+        }
+        ring.done_reading();
+        // the sum's barrier also says that every thread has read the stage
+        const A m = group_sum<G>(part.sum(), buf, slot) / (A)cols;
+        if (t == 0 && row + stages * step < rows) ring.fill(ring.at, x + (row + stages * step) * ldx);
+        ring.advance();
+        const A r = rsqrt_acc<A>(group_sum<G>(part.centre(m), buf, slot) / (A)cols + (A)eps);
+        if (t == 0) {
+            if (mean) mean[row] = m;
+            if (rstd) rstd[row] = r;
+        }
+        part.store(r, gamma, beta, y + row * ldy);
     }
 }
 
@@ -161,6 +292,71 @@ layer_norm_long_kernel(const T *x, long ldx, const W *__restrict__ gamma, const 
     }
 }
 
+// One row of the backward pass as a thread sees it, and its share of the sums over rows.
+template <class T, class W, int VEC, int G, int CH> struct BackPart {
+    using A = acc_t<T>;
+    using P = SimdOf<T, VEC>;
+    static constexpr int PV = VEC / kPack<VEC>;
+    P dg[CH][PV], db[CH][PV], xh[CH][PV], g[CH][PV];
+    int left;
+    __device__ __forceinline__ BackPart(int cols, int t) : left(cols - t * VEC) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < PV; ++i) dg[c][i] = db[c][i] = P::splat(A(0));
+    }
+    __device__ __forceinline__ bool has(int c) const { return c * G * VEC < left; }
+    // sums of g and g xh over this thread's elements, from functions that give chunk c of x and dy
+    template <class X, class D>
+    __device__ __forceinline__ void take(A m, A r, const W *gamma, X &&x_at, D &&d_at, A &s1, A &s2) {
+        const P scale = P::splat(r), shift = P::splat(-m);
+        P a = P::splat(A(0)), b = a;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+            if (has(c)) {
+                P d[PV], w[PV];
+                widen(x_at(c), xh[c]);
+                widen(d_at(c), d);
+                if (gamma) widen(load_vec<W, VEC>(gamma + c * G * VEC), w);
+#pragma unroll
+                for (int i = 0; i < PV; ++i) {
+                    xh[c][i] = mul(add(xh[c][i], shift), scale);
+                    dg[c][i] = fma(d[i], xh[c][i], dg[c][i]);
+                    db[c][i] = add(db[c][i], d[i]);
+                    g[c][i] = gamma ? mul(d[i], w[i]) : d[i];
+                    a = add(a, g[c][i]);
+                    b = fma(g[c][i], xh[c][i], b);
+                }
+            }
+        s1 = a.sum();
+        s2 = b.sum();
+    }
+    // dx = r (g - s1 - xh s2)
+    __device__ __forceinline__ void store(A r, A s1, A s2, T *dx) const {
+        const P scale = P::splat(r), back1 = P::splat(-s1), back2 = P::splat(-s2);
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+            if (has(c)) {
+                P o[PV];
+#pragma unroll
+                for (int i = 0; i < PV; ++i) o[i] = mul(fma(xh[c][i], back2, add(g[c][i], back1)), scale);
+                store_vec<T, VEC>(dx + c * G * VEC, narrowed<T, VEC>(o));
+            }
+    }
+    // this thread's columns of the block's partial sums
+    __device__ __forceinline__ void flush(A *pg, A *pb) const {
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+            if (has(c)) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    pg[c * G * VEC + e] = dg[c][e / kPack<VEC>].get(e % kPack<VEC>);
+                    pb[c * G * VEC + e] = db[c][e / kPack<VEC>].get(e % kPack<VEC>);
+                }
+            }
+    }
+};
+
 template <class T, class W, int VEC, int G>
 __global__ void __launch_bounds__(norm_threads<G>, norm_threads<G> <= 256 ? 2 : 1)
 layer_norm_backward_kernel(const T *dy, long lddy, const T *x, long ldx, const W *__restrict__ gamma,
@@ -168,106 +364,116 @@ layer_norm_backward_kernel(const T *dy, long lddy, const T *x, long ldx, const W
                            acc_t<T> *partial, long rows, int cols) {
     using A = acc_t<T>;
     constexpr int CH = N_ELEMS / VEC;
-    constexpr int THREADS = norm_threads<G>;
-    constexpr int RPB = THREADS / G;
+    constexpr int RPB = norm_threads<G> / G;   // rows a block works on at a time
     __shared__ A buf[G > 32 ? 4 * (G / 32) : 1];
-    const int t = threadIdx.x % G;
+    const int t = threadIdx.x % G, group = threadIdx.x / G;
     const long step = (long)gridDim.x * RPB;
-    long row = (long)blockIdx.x * RPB + threadIdx.x / G;
+    long row = (long)blockIdx.x * RPB + group;
     int slot = 0;
-    A dg[N_ELEMS], db[N_ELEMS];
-#pragma unroll
-    for (int i = 0; i < N_ELEMS; ++i) dg[i] = db[i] = 0;
+    x += t * VEC;
+    dy += t * VEC;
+    dx += t * VEC;
+    if (gamma) gamma += t * VEC;
+    BackPart<T, W, VEC, G, CH> part(cols, t);
     Vec<T, VEC> nx[CH], nd[CH];
     if (row < rows) {
 #pragma unroll
         for (int c = 0; c < CH; ++c)
-            if ((c * G + t) * VEC < cols) {
-                nx[c] = load_vec<T, VEC>(x + row * ldx + (c * G + t) * VEC);
-                nd[c] = load_vec<T, VEC>(dy + row * lddy + (c * G + t) * VEC);
+            if (part.has(c)) {
+                nx[c] = load_vec<T, VEC>(x + row * ldx + c * G * VEC);
+                nd[c] = load_vec<T, VEC>(dy + row * lddy + c * G * VEC);
             }
     }
     for (; row < rows; row += step) {
-        const A m = mean[row], r = rstd[row];
-        A xh[N_ELEMS], g[N_ELEMS];
-        A s1 = 0, s2 = 0;
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int at = (c * G + t) * VEC;
-            if (at < cols) {
-                Vec<W, VEC> w;
-                if (gamma) w = load_vec<W, VEC>(gamma + at);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const int i = c * VEC + e;
-                    const A d = to_acc<A>(nd[c].v[e]);
-                    xh[i] = (to_acc<A>(nx[c].v[e]) - m) * r;
-                    dg[i] += d * xh[i];
-                    db[i] += d;
-                    g[i] = gamma ? d * to_acc<A>(w.v[e]) : d;
-                    s1 += g[i];
-                    s2 += g[i] * xh[i];
-                }
-            }
-        }
+        const A r = rstd[row];
+        A s1, s2;
+        part.take(mean[row], r, gamma, [&](int c) { return nx[c]; }, [&](int c) { return nd[c]; }, s1, s2);
         if (row + step < rows) {
 #pragma unroll
             for (int c = 0; c < CH; ++c)
-                if ((c * G + t) * VEC < cols) {
-                    nx[c] = load_vec<T, VEC>(x + (row + step) * ldx + (c * G + t) * VEC);
-                    nd[c] = load_vec<T, VEC>(dy + (row + step) * lddy + (c * G + t) * VEC);
+                if (part.has(c)) {
+                    nx[c] = load_vec<T, VEC>(x + (row + step) * ldx + c * G * VEC);
+                    nd[c] = load_vec<T, VEC>(dy + (row + step) * lddy + c * G * VEC);
                 }
         }
         group_sum2<G>(s1, s2, buf, slot);
-        s1 /= (A)cols;
-        s2 /= (A)cols;
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int at = (c * G + t) * VEC;
-            if (at < cols) {
-                Vec<T, VEC> o;
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const int i = c * VEC + e;
-                    o.v[e] = from_acc<T>(r * (g[i] - s1 - xh[i] * s2));
-                }
-                store_vec<T, VEC>(dx + row * lddx + at, o);
-            }
-        }
+        part.store(r, s1 / (A)cols, s2 / (A)cols, dx + row * lddx);
     }
     if (!partial) return;
-    A *pg = partial + (long)blockIdx.x * 2 * cols, *pb = pg + cols;
-    if (G == 32) {
-        // the block's warps hold the same columns: added in warp order through shared memory
-        __shared__ A sg[G == 32 ? G * N_ELEMS : 1], sb[G == 32 ? G * N_ELEMS : 1];
-        for (int w = 0; w < RPB; ++w) {
-            if ((int)threadIdx.x / G == w) {
-#pragma unroll
-                for (int i = 0; i < N_ELEMS; ++i) {
-                    A *pgs = sg + i * G + t, *pbs = sb + i * G + t;
-                    *pgs = w ? *pgs + dg[i] : dg[i];
-                    *pbs = w ? *pbs + db[i] : db[i];
-                }
-            }
-            __syncthreads();
-        }
-        if ((int)threadIdx.x / G != 0) return;
-#pragma unroll
-        for (int i = 0; i < N_ELEMS; ++i) {
-            dg[i] = sg[i * G + t];
-            db[i] = sb[i * G + t];
-        }
+    A *pg = partial + (long)blockIdx.x * 2 * cols + t * VEC, *pb = pg + cols;
+    if (G > 32) {
+        part.flush(pg, pb);
+        return;
     }
+    // the block's warps hold the same columns: added in warp order through shared memory
+    __shared__ A sg[G == 32 ? G * N_ELEMS : 1], sb[G == 32 ? G * N_ELEMS : 1];
+    for (int w = 0; w < RPB; ++w) {
+        if (group == w) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+            for (int c = 0; c < CH; ++c)
+                if (part.has(c)) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const int at = (c * G + t) * VEC + e;
-            if (at < cols) {
-                pg[at] = dg[c * VEC + e];
-                pb[at] = db[c * VEC + e];
-            }
+                    for (int e = 0; e < VEC; ++e) {
+                        const int i = c * G * VEC + t * VEC + e;
+                        const A a = part.dg[c][e / kPack<VEC>].get(e % kPack<VEC>), b = part.db[c][e / kPack<VEC>].get(e % kPack<VEC>);
+                        sg[i] = w ? sg[i] + a : a;
+                        sb[i] = w ? sb[i] + b : b;
+                    }
+                }
         }
+        __syncthreads();
+    }
+    pg -= t * VEC;
+    pb -= t * VEC;
+    for (int i = threadIdx.x; i < cols; i += norm_threads<G>) {
+        pg[i] = sg[i];
+        pb[i] = sb[i];
+    }
+}
+
+template <class T, class W, int VEC, int G>
+__global__ void __launch_bounds__(G, 768 / G > 0 ? 768 / G : 1)
+layer_norm_backward_ring_kernel(const T *dy, long lddy, const T *x, long ldx, const W *__restrict__ gamma,
+                                const acc_t<T> *__restrict__ mean, const acc_t<T> *__restrict__ rstd, T *dx, long lddx,
+                                acc_t<T> *partial, long rows, int cols, int stages, int *err) {
+    using A = acc_t<T>;
+    constexpr int CH = N_ELEMS / VEC;
+    extern __shared__ __align__(16) unsigned char ring_raw[];
+    __shared__ unsigned long long bars[kRingMax];
+    __shared__ A buf[4 * (G / 32)];
+    const int t = threadIdx.x, bytes = cols * (int)sizeof(T);
+    const long step = gridDim.x;
+    int slot = 0;
+    RowRing ring(ring_raw, bars, stages, 2 * bytes);
+    ring.init();
+    if (t == 0)
+        for (int i = 0; i < stages; ++i) {
+            const long r = blockIdx.x + i * step;
+            if (r < rows) ring.fill2(i, x + r * ldx, dy + r * lddy);
+        }
+    dx += t * VEC;
+    if (gamma) gamma += t * VEC;
+    BackPart<T, W, VEC, G, CH> part(cols, t);
+    for (long row = blockIdx.x; row < rows; row += step) {
+        const A m = mean[row], r = rstd[row];
+        if (!ring.wait()) {
+            if (t == 0) atomicExch(err, 1);
+            return;
+        }
+        const T *xs = (const T *)ring.data() + t * VEC, *ds = (const T *)(ring.data() + bytes) + t * VEC;
+        A s1, s2;
+        part.take(m, r, gamma, [&](int c) { return load_vec<T, VEC>(xs + c * G * VEC); },
+                  [&](int c) { return load_vec<T, VEC>(ds + c * G * VEC); }, s1, s2);
+        ring.done_reading();
+        group_sum2<G>(s1, s2, buf, slot);
+        if (t == 0 && row + stages * step < rows)
+            ring.fill2(ring.at, x + (row + stages * step) * ldx, dy + (row + stages * step) * lddy);
+        ring.advance();
+        part.store(r, s1 / (A)cols, s2 / (A)cols, dx + row * lddx);
+    }
+    if (!partial) return;
+    A *pg = partial + (long)blockIdx.x * 2 * cols + t * VEC;
+    part.flush(pg, pg + cols);
 }
 
 // Column sums for rows too long for registers: a block takes 256 columns and every gridDim.y-th row.
@@ -349,6 +555,16 @@ int blocks_for(long rows, int g, int threads_per_sm) {
     return (int)(need < room ? need : room);
 }
 constexpr int kBackThreads = 512;        // resident threads per SM of the backward kernel
+constexpr int kRingThreads = 768;        // ... of its ring form
+// Stages of a ring: as many rows as fit the block's share of 200 KB, at least 2 and at most 8 (0: too wide).
+int ring_stages(int threads, int threads_per_sm, long bytes) {
+    const int blocks = threads_per_sm / threads > 0 ? threads_per_sm / threads : 1;
+    const long s = 200 * 1024 / blocks / bytes;
+    return s < 2 ? 0 : s > kRingMax ? kRingMax : (int)s;
+}
+template <class K> void allow_shared(K kernel, size_t bytes) {
+    FITRE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+}
 constexpr int kLongSplit = 64;           // row splits of the column sums of long rows
 
 template <class T, class W, int VEC>
@@ -359,12 +575,35 @@ void forward_as(fitre_context *ctx, const NormArgs &a) {
     T *y = (T *)a.y;
     const W *gm = (const W *)a.gamma, *bt = (const W *)a.beta;
     A *mean = (A *)a.mean, *rstd = (A *)a.rstd;
+    if (a.cols <= 32 * N_WIDE) {
+        layer_norm_warp_kernel<T, W, VEC><<<(unsigned)((a.rows + 7) / 8), 256, 0, ctx->stream>>>(
+            x, a.ldx, gm, bt, y, a.ldy, mean, rstd, a.rows, a.cols, a.eps);
+        check_launch(ctx, "layer_norm_warp_kernel");
+        return;
+    }
     const int blocks = blocks_for(a.rows, g ? g : 1024, sizeof(T) == 8 ? 512 : 1024);
+    const long bytes = (long)a.cols * sizeof(T);
+    const int stages = VEC > 1 && g ? ring_stages(g, 1024, bytes) : 0;
+    if constexpr (VEC > 1) if (stages) {
+        const int room = blocks_for(a.rows, g, 1024);
 #define NORM_LAUNCH(G)                                                                                       \
-    layer_norm_kernel<T, W, VEC, G><<<blocks, norm_threads<G>, 0, ctx->stream>>>(                          \
+    allow_shared(layer_norm_ring_kernel<T, W, VEC, G>, stages * bytes);                                      \
+    layer_norm_ring_kernel<T, W, VEC, G><<<room, G, stages * bytes, ctx->stream>>>(                          \
+        x, a.ldx, gm, bt, y, a.ldy, mean, rstd, a.rows, a.cols, a.eps, stages, (int *)(ctx->dscal + 4000))
+        switch (g) {
+            case 128: NORM_LAUNCH(128); break;
+            case 256: NORM_LAUNCH(256); break;
+            case 512: NORM_LAUNCH(512); break;
+            default: NORM_LAUNCH(1024); break;
+        }
+#undef NORM_LAUNCH
+        check_launch(ctx, "layer_norm_ring_kernel");
+        return;
+    }
+#define NORM_LAUNCH(G)                                                                                       \
+    layer_norm_kernel<T, W, VEC, G><<<blocks, G, 0, ctx->stream>>>(                          \
         x, a.ldx, gm, bt, y, a.ldy, mean, rstd, a.rows, a.cols, a.eps)
     switch (g) {
-        case 32: NORM_LAUNCH(32); break;
         case 128: NORM_LAUNCH(128); break;
         case 256: NORM_LAUNCH(256); break;
         case 512: NORM_LAUNCH(512); break;
@@ -389,6 +628,24 @@ void backward_as(fitre_context *ctx, const NormArgs &a) {
     const A *mean = (const A *)a.mean, *rstd = (const A *)a.rstd;
     A *partial = a.dgamma || a.dbeta ? (A *)a.scratch : nullptr;
     int blocks = blocks_for(a.rows, g ? g : 1024, kBackThreads);
+    const long bytes = 2l * a.cols * sizeof(T);
+    const int stages = VEC > 1 && g > 32 ? ring_stages(g, kRingThreads, bytes) : 0;
+    if constexpr (VEC > 1) if (stages) {
+        blocks = blocks_for(a.rows, g, kRingThreads);
+#define NORM_LAUNCH(G)                                                                                       \
+    allow_shared(layer_norm_backward_ring_kernel<T, W, VEC, G>, stages * bytes);                             \
+    layer_norm_backward_ring_kernel<T, W, VEC, G><<<blocks, G, stages * bytes, ctx->stream>>>(               \
+        dy, a.lddy, x, a.ldx, gm, mean, rstd, dx, a.lddx, partial, a.rows, a.cols, stages, (int *)(ctx->dscal + 4000))
+        switch (g) {
+            case 128: NORM_LAUNCH(128); break;
+            case 256: NORM_LAUNCH(256); break;
+            case 512: NORM_LAUNCH(512); break;
+            default: NORM_LAUNCH(1024); break;
+        }
+#undef NORM_LAUNCH
+        check_launch(ctx, "layer_norm_backward_ring_kernel");
+    }
+    if (!stages) {
 #define NORM_LAUNCH(G)                                                                                       \
     layer_norm_backward_kernel<T, W, VEC, G><<<blocks, norm_threads<G>, 0, ctx->stream>>>(                 \
         dy, a.lddy, x, a.ldx, gm, mean, rstd, dx, a.lddx, partial, a.rows, a.cols)
@@ -416,6 +673,7 @@ void backward_as(fitre_context *ctx, const NormArgs &a) {
     }
 #undef NORM_LAUNCH
     check_launch(ctx, "layer_norm_backward_kernel");
+    }
     if (partial) {
         layer_norm_reduce_kernel<W, A><<<(2 * a.cols + 31) / 32, 1024, 0, ctx->stream>>>(
             partial, blocks, a.cols, (W *)a.dgamma, (W *)a.dbeta);
@@ -460,7 +718,7 @@ void norm_dispatch(fitre_context *ctx, const NormArgs &a, bool back) {
 
 long layer_norm_backward_scratch(long rows, long cols) {
     const int g = cols <= 1024 * N_ELEMS ? group_for((int)cols) : 0;
-    const long parts = g ? blocks_for(rows, g, kBackThreads) : (rows < kLongSplit ? rows : kLongSplit);
+    const long parts = g ? blocks_for(rows, g, kRingThreads) : (rows < kLongSplit ? rows : kLongSplit);
     return parts * 2 * cols * (long)sizeof(double);
 }
 void layer_norm_forward(fitre_context *ctx, const NormArgs &a) { norm_dispatch(ctx, a, false); }

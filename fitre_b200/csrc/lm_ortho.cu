@@ -22,45 +22,65 @@ namespace {
 
 constexpr float kScale = 1024.0f;   // 2^10: what the stored iterates are multiplied by
 
-// sum of squares of a part of each matrix, in fp64 (squares of fp32 values overflow fp32)
-constexpr int O_PARTS = 64;
-template <class T>
+// Sum over the block's 256 threads, in a fixed order; every thread gets it.
+__device__ __forceinline__ double block_sum(double q, double *s) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = q;
+    __syncthreads();
+    q = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) q += s[w];
+    return q;
+}
+
+// Sums of squares of each matrix's parts, in fp64 (squares of fp32 values overflow fp32): part p holds every
+// gridDim.x-th row.
+template <class T, int VEC>
 __global__ void __launch_bounds__(256)
 ortho_norm_kernel(const T *in, long ld, long bstride, int rows, int cols, double *partial) {
     __shared__ double s[8];
     const T *m = in + blockIdx.y * bstride;
     double q = 0;
     for (int r = blockIdx.x; r < rows; r += gridDim.x)
-        for (int c = threadIdx.x; c < cols; c += 256) {
-            const double v = (double)to_acc<acc_t<T>>(m[r * ld + c]);
-            q += v * v;
-        }
+#pragma unroll 4
+        for (int c = threadIdx.x * VEC; c < cols; c += 256 * VEC) {
+            const Vec<T, VEC> x = load_vec<T, VEC>(m + r * ld + c);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = q;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < 8; ++w) q += s[w];
-        partial[blockIdx.y * O_PARTS + blockIdx.x] = q;
-    }
+            for (int e = 0; e < VEC; ++e) {
+                const double v = (double)to_acc<acc_t<T>>(x.v[e]);
+                q += v * v;
+            }
+        }
+    q = block_sum(q, s);
+    if (threadIdx.x == 0) partial[(long)blockIdx.y * gridDim.x + blockIdx.x] = q;
 }
 
-template <class T>
+// The first iterate, as a pair of fp16 matrices.
+template <class T, int VEC>
 __global__ void __launch_bounds__(256)
 ortho_scale_kernel(const T *in, long ld, long bstride, int rows, int cols, const double *__restrict__ partial, int parts,
                    double eps, __half *hi, __half *lo, long ldo, long ostride) {
+    __shared__ double s[8];
     double q = 0;
-    for (int i = 0; i < parts; ++i) q += partial[blockIdx.y * O_PARTS + i];
-    const double f = (double)kScale / (sqrt(q) + eps);
+    for (int i = threadIdx.x; i < parts; i += 256) q += partial[(long)blockIdx.y * parts + i];
+    const double f = (double)kScale / (sqrt(block_sum(q, s)) + eps);
     const T *m = in + blockIdx.y * bstride;
     hi += blockIdx.y * ostride;
     lo += blockIdx.y * ostride;
     for (int r = blockIdx.x; r < rows; r += gridDim.x)
-        for (int c = threadIdx.x; c < cols; c += 256) {
-            const float v = (float)((double)to_acc<acc_t<T>>(m[r * ld + c]) * f);
-            const __half h = __float2half_rn(v);
-            hi[r * ldo + c] = h;
-            lo[r * ldo + c] = __float2half_rn(v - __half2float(h));
+#pragma unroll 2
+        for (int c = threadIdx.x * VEC; c < cols; c += 256 * VEC) {
+            const Vec<T, VEC> x = load_vec<T, VEC>(m + r * ld + c);
+            Vec<__half, VEC> h, l;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float v = (float)((double)to_acc<acc_t<T>>(x.v[e]) * f);
+                h.v[e] = __float2half_rn(v);
+                l.v[e] = __float2half_rn(v - __half2float(h.v[e]));
+            }
+            store_vec<__half, VEC>(hi + r * ldo + c, h);
+            store_vec<__half, VEC>(lo + r * ldo + c, l);
         }
 }
 
@@ -177,6 +197,7 @@ long up128(long bytes) { return (bytes + 127) / 128 * 128; }
 
 struct Plan {
     int rows, cols, small;   // small: the order of A and B
+    int parts;               // blocks that sum one matrix's squares
     int batch;
     bool tall;
     long ldx, xs, lda, as;
@@ -189,6 +210,8 @@ struct Plan {
         small = tall ? cols : rows;
         ldx = up8(cols), xs = up128(2 * ldx * rows) / 2;
         lda = up8(small), as = up128(2 * lda * small) / 2;
+        parts = 8 * kLmSms / batch < rows ? 8 * kLmSms / batch : rows;
+        parts = parts > 0 ? parts : 1;
         char *p = (char *)a.scratch;
         auto take = [&](long bytes) {
             char *q = p;
@@ -201,7 +224,7 @@ struct Plan {
         A = (__half *)take(2 * as * batch);
         B = (__half *)take(2 * as * batch);
         diag = (float *)take(4 * (long)small * batch);
-        partial = (double *)take(8 * O_PARTS * (long)batch);
+        partial = (double *)take(8 * (long)parts * batch);
         bytes = p - (char *)a.scratch;
     }
     long bytes;
@@ -239,15 +262,22 @@ void iterate(fitre_context *ctx, const Plan &pl, const __half *x, T *out, long l
     }
 }
 
+template <class T, int VEC>
+void start_as(fitre_context *ctx, const OrthoArgs &a, const Plan &pl) {
+    const dim3 grid(pl.parts, pl.batch);
+    ortho_norm_kernel<T, VEC><<<grid, 256, 0, ctx->stream>>>((const T *)a.in, a.ldi, a.istride, pl.rows, pl.cols,
+                                                             pl.partial);
+    check_launch(ctx, "ortho_norm_kernel");
+    ortho_scale_kernel<T, VEC><<<grid, 256, 0, ctx->stream>>>((const T *)a.in, a.ldi, a.istride, pl.rows, pl.cols,
+                                                              pl.partial, pl.parts, a.eps, pl.x[0], pl.lo, pl.ldx, pl.xs);
+    check_launch(ctx, "ortho_scale_kernel");
+}
 template <class T>
 void start(fitre_context *ctx, const OrthoArgs &a, const Plan &pl) {
-    const int parts = pl.rows < O_PARTS ? pl.rows : O_PARTS;
-    ortho_norm_kernel<T><<<dim3(parts, pl.batch), 256, 0, ctx->stream>>>((const T *)a.in, a.ldi, a.istride, pl.rows,
-                                                                         pl.cols, pl.partial);
-    check_launch(ctx, "ortho_norm_kernel");
-    ortho_scale_kernel<T><<<dim3(pl.rows < 1024 ? pl.rows : 1024, pl.batch), 256, 0, ctx->stream>>>(
-        (const T *)a.in, a.ldi, a.istride, pl.rows, pl.cols, pl.partial, parts, a.eps, pl.x[0], pl.lo, pl.ldx, pl.xs);
-    check_launch(ctx, "ortho_scale_kernel");
+    constexpr int VEC = 16 / sizeof(T);
+    const bool wide = aligned16(a.in) && pl.cols % VEC == 0 && (a.ldi * (long)sizeof(T)) % 16 == 0 &&
+                      (a.istride * (long)sizeof(T)) % 16 == 0;
+    wide ? start_as<T, VEC>(ctx, a, pl) : start_as<T, 1>(ctx, a, pl);
 }
 
 }  // namespace

@@ -1,0 +1,59 @@
+// A ring of buffers in shared memory that bulk copies fill with rows of global memory (rows on 16-byte
+// boundaries, whole multiples of 16 bytes).  One thread fills, all threads of the block read; a
+// block-wide barrier between the last read of a stage and its refill is the caller's.
+#pragma once
+
+#include "tma_util.cuh"
+
+namespace fitre {
+namespace {
+
+constexpr int kRingMax = 8;
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
+struct RowRing {
+    unsigned char *base;
+    unsigned long long *bars;
+    int stages, bytes, at = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ RowRing(unsigned char *b, unsigned long long *m, int s, int n)
+        : base(b), bars(m), stages(s), bytes(n) {}
+    __device__ __forceinline__ void init() {
+        if (threadIdx.x == 0) {
+            for (int i = 0; i < stages; ++i) mbar_init(smem_u32(bars + i), 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ void fill(int i, const void *src) {
+        const uint32_t bar = smem_u32(bars + i);
+        mbar_expect_tx(bar, bytes);
+        bulk_load(smem_u32(base + (size_t)i * bytes), src, bytes, bar);
+    }
+    // two rows of equal length, one after the other
+    __device__ __forceinline__ void fill2(int i, const void *a, const void *b) {
+        const uint32_t bar = smem_u32(bars + i), dst = smem_u32(base + (size_t)i * bytes);
+        mbar_expect_tx(bar, bytes);
+        bulk_load(dst, a, bytes / 2, bar);
+        bulk_load(dst + bytes / 2, b, bytes / 2, bar);
+    }
+    // false: the bounded wait ran out
+    __device__ __forceinline__ bool wait() const { return mbar_wait(smem_u32(bars + at), phase); }
+    __device__ __forceinline__ const unsigned char *data() const { return base + (size_t)at * bytes; }
+    // after a thread's last read of the stage, before the block's barrier
+    __device__ __forceinline__ void done_reading() const { release_stage_reads(); }
+    __device__ __forceinline__ void advance() {
+        if (++at == stages) {
+            at = 0;
+            phase ^= 1;
+        }
+    }
+};
+
+}  // namespace
+}  // namespace fitre
