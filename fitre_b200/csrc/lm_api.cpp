@@ -302,6 +302,7 @@ int fitre_orthogonalize_update(fitre_context *ctx, int dtype, const void *update
         need(std::isfinite(coef[0]) && std::isfinite(coef[1]) && std::isfinite(coef[2]),
              "orthogonalised update: coefficients not finite");
         if (batch == 0) return;
+        settle_stride(ldu, rows, cols), settle_stride(ldo, rows, cols);
         need_matrix(update, ldu, rows, cols, dtype, "update");
         need_matrix(out, ldo, rows, cols, FITRE_DTYPE_BF16, "out");
         const long spanu = rows > 1 ? (rows - 1) * ldu + cols : cols, spano = rows > 1 ? (rows - 1) * ldo + cols : cols;

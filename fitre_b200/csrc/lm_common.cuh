@@ -88,6 +88,24 @@ template <class T, int VEC> __device__ __forceinline__ void store_vec(T *p, cons
     *reinterpret_cast<Vec<T, VEC> *>(p) = v;
 }
 
+// A kernel that follows another of this library in the same call may start while that one drains: it has to
+// wait here before it touches memory.  Without the launch attribute (launch_after below) both are no-ops.
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <class... P, class... A>
+void launch_after(cudaStream_t stream, void (*kernel)(P...), dim3 grid, int threads, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    FITRE_CUDA(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
+}
+
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 inline int dtype_bytes(int dtype) { return dtype == FITRE_DTYPE_F64 ? 8 : dtype == FITRE_DTYPE_F32 ? 4 : 2; }
 

@@ -39,28 +39,25 @@ __device__ __forceinline__ float act_slope(int act, float g) {
 template <class T>
 struct GatedEpi {
     struct Params {
-        T *h, *g, *u;
-        long ldh, ldg, ldu;
-        int M, F, act;
-        bool wide;
+        Output<T> h, g, u;
+        int act;
     };
     static constexpr bool kTwoMaps = true;
     template <int BN>
-    static __device__ __forceinline__ void store(const Params &p, TileAt at, int row, uint32_t tmem) {
+    static __device__ __forceinline__ void store(const Params &p, TileAt at, int row0, uint32_t tmem, Stager &st) {
+        // columns: the tile's gates, then as many ups
+        const int width = at.half < 0 ? BN / 2 : BN / 4, first = at.n * (BN / 2) + (at.half > 0 ? BN / 4 : 0);
+        if (row0 >= p.h.rows) return;
 #pragma unroll 1
-        for (int c = 0; c < BN / 2; c += 32) {
-            const int col = at.n * (BN / 2) + c;
-            if (col >= p.F) break;
-            float g[32], u[32];
-            tmem_load32(tmem + c, g);
-            tmem_load32(tmem + BN / 2 + c, u);
-            if (row < p.M) {
-                if (p.g) store_row32(p.g + (long)row * p.ldg, col, p.F, p.wide, g);
-                if (p.u) store_row32(p.u + (long)row * p.ldu, col, p.F, p.wide, u);
+        for (int c = 0; c < width && first + c < p.h.cols; c += 64) {
+            float g[64], u[64];
+            tmem_load64(tmem + c, g);
+            tmem_load64(tmem + width + c, u);
+            if (p.g.out) st.put(p.g, row0, first + c, 0, g);
+            if (p.u.out) st.put(p.u, row0, first + c, 0, u);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) u[i] *= act_value(p.act, g[i]);
-                store_row32(p.h + (long)row * p.ldh, col, p.F, p.wide, u);
-            }
+            for (int i = 0; i < 64; ++i) u[i] *= act_value(p.act, g[i]);
+            st.put(p.h, row0, first + c, 0, u);
         }
     }
 };
@@ -108,14 +105,18 @@ gated_few_kernel(const T *__restrict__ x, long ldx, const T *__restrict__ wg, lo
     }
 }
 
-// dg and du, side by side in scratch ([2][T][ld]).
+// dg and du, side by side in scratch ([2][T][ld], zeros beyond F).
 template <class T, int VEC>
 __global__ void __launch_bounds__(256)
 gated_slopes_kernel(const T *dh, long lddh, const T *g, long ldg, const T *u, long ldu, T *out, long ld, long half,
                     int F, int act) {
+    let_next_kernel_start();
     const long row = blockIdx.y;
     const int at = (blockIdx.x * 256 + threadIdx.x) * VEC;
-    if (at >= F) return;
+    if (at >= F) {
+        if (VEC == 1 && at < ld) out[row * ld + at] = out[half + row * ld + at] = from_acc<T>(0.0f);
+        return;
+    }
     const Vec<T, VEC> a = load_vec<T, VEC>(dh + row * lddh + at), b = load_vec<T, VEC>(g + row * ldg + at),
                       c = load_vec<T, VEC>(u + row * ldu + at);
     Vec<T, VEC> dg, du;
@@ -129,12 +130,12 @@ gated_slopes_kernel(const T *dh, long lddh, const T *g, long ldg, const T *u, lo
     store_vec<T, VEC>(out + half + row * ld + at, du);
 }
 
-// A matrix whose rows TMA cannot read, copied to rows that it can.
+// A matrix whose rows TMA cannot read, copied to rows that it can, padded with zeros.
 template <class T>
 __global__ void __launch_bounds__(256)
 align_rows_kernel(const T *in, long ld, T *out, long ldo, long rows, int cols) {
     for (long row = blockIdx.x; row < rows; row += gridDim.x)
-        for (int c = threadIdx.x; c < cols; c += 256) out[row * ldo + c] = in[row * ld + c];
+        for (int c = threadIdx.x; c < ldo; c += 256) out[row * ldo + c] = c < cols ? in[row * ld + c] : from_acc<T>(0.0f);
 }
 
 long up8(long n) { return (n + 7) / 8 * 8; }
@@ -177,13 +178,15 @@ template <class T> constexpr int fmt_of = sizeof(T) && std::is_same<T, __half>::
 template <class T, int CG, int BN>
 void forward_tiles(fitre_context *ctx, const GatedArgs &a, const Operands<T> &o) {
     GemmArgs<typename GatedEpi<T>::Params> g = {};
-    const int T_ = (int)a.tokens, D = (int)a.width, F = (int)a.hidden;
+    const int T_ = (int)a.tokens, D = (int)up8(a.width), F = (int)a.hidden;
     gemm_map(&g.a[0], o.x, D, T_, 1, o.ldx, 0, a_box<CG, BN, false>, fmt_of<T>);
     gemm_map(&g.b[0], o.wg, D, F, 1, o.ldwg, 0, b_box<CG, BN, false, true>, fmt_of<T>);
     gemm_map(&g.b[1], o.wu, D, F, 1, o.ldwu, 0, b_box<CG, BN, false, true>, fmt_of<T>);
-    const bool wide = tma_readable(a.h, a.ldh) && (!a.g || tma_readable(a.g, a.ldg)) && (!a.u || tma_readable(a.u, a.ldu));
-    g.epi = {(T *)a.h, (T *)a.g, (T *)a.u, a.ldh, a.ldg, a.ldu, T_, F, a.act, wide};
-    gemm_launch<CG, BN, false, false, GatedEpi<T>>(ctx, g, T_, F, 1, false, D, 1, fmt_of<T>, "gated_tiles_kernel");
+    g.epi.h = gemm_output<T>(a.h, F, T_, 1, a.ldh, 0, fmt_of<T>);
+    g.epi.g = gemm_output<T>(a.g, F, T_, 1, a.ldg, 0, fmt_of<T>);
+    g.epi.u = gemm_output<T>(a.u, F, T_, 1, a.ldu, 0, fmt_of<T>);
+    g.epi.act = a.act;
+    gemm_launch<CG, BN, false, false, GatedEpi<T>>(ctx, g, T_, F, 1, false, D, 1, fmt_of<T>, "gated_tiles_kernel", false);
 }
 
 // Whether a product has tiles enough for the SM pairs' 256-row tiles; below, 128-row tiles on single SMs
@@ -227,23 +230,24 @@ template <class T, int CG, int BN>
 void input_gradient(fitre_context *ctx, const GatedArgs &a, const Operands<T> &o, const T *slopes, long ld, long half) {
     GemmArgs<typename StoreEpi<T>::Params> g = {};
     const int T_ = (int)a.tokens, D = (int)a.width, F = (int)a.hidden;
-    gemm_map(&g.a[0], slopes, F, T_, 1, ld, 0, a_box<CG, BN, false>, fmt_of<T>);
-    gemm_map(&g.a[1], slopes + half, F, T_, 1, ld, 0, a_box<CG, BN, false>, fmt_of<T>);
-    gemm_map(&g.b[0], o.wg, D, F, 1, o.ldwg, 0, b_box<CG, BN, true, false>, fmt_of<T>);
-    gemm_map(&g.b[1], o.wu, D, F, 1, o.ldwu, 0, b_box<CG, BN, true, false>, fmt_of<T>);
-    g.epi = {{(T *)a.dx, nullptr}, {a.lddx, 0}, T_, D, tma_readable(a.dx, a.lddx)};
-    gemm_launch<CG, BN, false, true, StoreEpi<T>>(ctx, g, T_, D, 1, false, F, 2, fmt_of<T>, "gated_input_gradient_kernel");
+    gemm_map(&g.a[0], slopes, ld, T_, 1, ld, 0, a_box<CG, BN, false>, fmt_of<T>);
+    gemm_map(&g.a[1], slopes + half, ld, T_, 1, ld, 0, a_box<CG, BN, false>, fmt_of<T>);
+    gemm_map(&g.b[0], o.wg, up8(D), F, 1, o.ldwg, 0, b_box<CG, BN, true, false>, fmt_of<T>);
+    gemm_map(&g.b[1], o.wu, up8(D), F, 1, o.ldwu, 0, b_box<CG, BN, true, false>, fmt_of<T>);
+    g.epi.out[0] = gemm_output<T>(a.dx, D, T_, 1, a.lddx, 0, fmt_of<T>);
+    gemm_launch<CG, BN, false, true, StoreEpi<T>>(ctx, g, T_, D, 1, false, F, 2, fmt_of<T>, "gated_input_gradient_kernel",
+                                                    a.width % 8 == 0);
 }
 template <class T, int CG, int BN>
 void weight_gradient(fitre_context *ctx, const GatedArgs &a, const Operands<T> &o, const T *slopes, long ld, long half) {
     GemmArgs<typename StoreEpi<T>::Params> g = {};
     const int T_ = (int)a.tokens, D = (int)a.width, F = (int)a.hidden;
-    gemm_map(&g.a[0], slopes, F, T_, 2, ld, half, a_box<CG, BN, true>, fmt_of<T>);
-    gemm_map(&g.b[0], o.x, D, T_, 1, o.ldx, 0, b_box<CG, BN, true, false>, fmt_of<T>);
+    gemm_map(&g.a[0], slopes, ld, T_, 2, ld, half, a_box<CG, BN, true>, fmt_of<T>);
+    gemm_map(&g.b[0], o.x, up8(D), T_, 1, o.ldx, 0, b_box<CG, BN, true, false>, fmt_of<T>);
     g.g.za = 1;
-    g.epi = {{(T *)a.dwg, (T *)a.dwu}, {a.lddwg, a.lddwu}, F, D,
-             tma_readable(a.dwg, a.lddwg) && tma_readable(a.dwu, a.lddwu)};
-    gemm_launch<CG, BN, true, true, StoreEpi<T>>(ctx, g, F, D, 2, false, T_, 1, fmt_of<T>, "gated_weight_gradient_kernel");
+    g.epi.out[0] = gemm_output<T>(a.dwg, D, F, 1, a.lddwg, 0, fmt_of<T>);
+    g.epi.out[1] = gemm_output<T>(a.dwu, D, F, 1, a.lddwu, 0, fmt_of<T>);
+    gemm_launch<CG, BN, true, true, StoreEpi<T>>(ctx, g, F, D, 2, false, T_, 1, fmt_of<T>, "gated_weight_gradient_kernel", true);
 }
 
 template <class T, int VEC>
@@ -251,7 +255,7 @@ void slopes_as(fitre_context *ctx, const GatedArgs &a, T *slopes, long ld, long 
     const long most = 65535;   // rows a grid's second dimension can count
     for (long r0 = 0; r0 < a.tokens; r0 += most) {
         const long n = a.tokens - r0 < most ? a.tokens - r0 : most;
-        gated_slopes_kernel<T, VEC><<<dim3((unsigned)((a.hidden + 256 * VEC - 1) / (256 * VEC)), (unsigned)n), 256, 0,
+        gated_slopes_kernel<T, VEC><<<dim3((unsigned)((ld + 256 * VEC - 1) / (256 * VEC)), (unsigned)n), 256, 0,
                                       ctx->stream>>>(
             (const T *)a.dh + r0 * a.lddh, a.lddh, (const T *)a.g + r0 * a.ldg, a.ldg, (const T *)a.u + r0 * a.ldu,
             a.ldu, slopes + r0 * ld, ld, half, (int)a.hidden, a.act);

@@ -8,7 +8,8 @@
 // Persistent kernel, warp-specialised:
 //   warp 0     one lane issues the TMA loads of a ring of stages (64 k per stage)
 //   warp 1     one lane issues tcgen05.mma; accumulators live in TMEM, two of them, so that
-//   warps 2-5  read and store one tile (Epi) while the next is being computed.
+//   warps 2-5  read and store one tile (Epi) while the next is being computed.  Each warp gathers 32 rows x 64
+//              columns in shared memory and sends them off as one TMA store: full cache lines, edges clipped.
 // CG = 2 pairs two SMs on a 256 x BN tile: each CTA loads its 128 rows of A and half of B's rows, so a byte
 // of B feeds twice the arithmetic; the even CTA's issuer drives both.  CG = 1 (128 x BN) is for products
 // with too few tiles to occupy the pairs.  Every wait is bounded; when one runs out, the CTA sets the
@@ -27,12 +28,13 @@ constexpr int G_KB = 64;   // k per stage: 128 bytes, one swizzle row
 // Which tiles there are and where their operands come from.
 struct TileGrid {
     int tilesM, tilesN;   // tiles of one product
-    int total;            // over all products of the batch
+    int whole;            // tiles over all products of the batch that are computed whole; those beyond, so few
+    int total;            // that they leave half of the last round idle, are computed as two halves each
     int per;              // tiles per product
     int triangle;         // 1: only tiles with column <= row (the product is symmetric)
     int kblocks, nseg;    // stages per segment, segments (map index = segment)
     int za, zb;           // 1: the batch index is the operand map's third coordinate
-    uint32_t idesc;
+    uint32_t idesc, idesc_half;
     int *err;
 };
 
@@ -120,24 +122,94 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
         asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
                      : "memory");
 }
-// 32 consecutive accumulator columns of this thread's row.
-__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
-    uint32_t r[32];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
-          "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
-          "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
-          "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(addr)
-        : "memory");
+// 64 consecutive accumulator columns of this thread's row.
+__device__ __forceinline__ void tmem_load64(uint32_t addr, float (&v)[64]) {
+    uint32_t r[64];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+            "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+            "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+            : "=r"(r[h * 32]), "=r"(r[h * 32 + 1]), "=r"(r[h * 32 + 2]), "=r"(r[h * 32 + 3]), "=r"(r[h * 32 + 4]),
+              "=r"(r[h * 32 + 5]), "=r"(r[h * 32 + 6]), "=r"(r[h * 32 + 7]), "=r"(r[h * 32 + 8]), "=r"(r[h * 32 + 9]),
+              "=r"(r[h * 32 + 10]), "=r"(r[h * 32 + 11]), "=r"(r[h * 32 + 12]), "=r"(r[h * 32 + 13]),
+              "=r"(r[h * 32 + 14]), "=r"(r[h * 32 + 15]), "=r"(r[h * 32 + 16]), "=r"(r[h * 32 + 17]),
+              "=r"(r[h * 32 + 18]), "=r"(r[h * 32 + 19]), "=r"(r[h * 32 + 20]), "=r"(r[h * 32 + 21]),
+              "=r"(r[h * 32 + 22]), "=r"(r[h * 32 + 23]), "=r"(r[h * 32 + 24]), "=r"(r[h * 32 + 25]),
+              "=r"(r[h * 32 + 26]), "=r"(r[h * 32 + 27]), "=r"(r[h * 32 + 28]), "=r"(r[h * 32 + 29]),
+              "=r"(r[h * 32 + 30]), "=r"(r[h * 32 + 31])
+            : "r"(addr + h * 32)
+            : "memory");
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+    for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
 }
+
+// Where a product's result goes: `map` for TMA stores (box 64 columns x 32 rows) where TMA can write it, else
+// `out` directly.
+template <class T> struct Output {
+    CUtensorMap map;
+    T *out;           // NULL: not wanted
+    long ld, stride;  // elements between rows, between matrices of a batch
+    int rows, cols;
+    int tma;
+};
+
+// An epilogue warp's two staging buffers of 32 rows x 128 bytes.
+struct Stager {
+    unsigned char *base;   // 1024-byte aligned
+    int turn;
+    // the next buffer, once its last store has read it
+    __device__ __forceinline__ unsigned char *next() {
+        if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        __syncwarp();
+        turn ^= 1;
+        return base + turn * 4096;
+    }
+    __device__ __forceinline__ static void send(const CUtensorMap *map, const unsigned char *buf, int x, int y, int z) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) {
+            asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map),
+                         "r"(smem_u32(buf)), "r"(x), "r"(y), "r"(z)
+                         : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+    }
+    __device__ __forceinline__ static void drain() {
+        if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+    // Stores 64 values of each lane's row: columns [col, col + 64), rows [row0, row0 + 32).
+    template <class T> __device__ __forceinline__ void put(const Output<T> &o, int row0, int col, int batch, const float (&v)[64]) {
+        const int lane = threadIdx.x & 31;
+        unsigned char *buf = next(), *mine = buf + lane * 128;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            Vec<T, 8> w;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w.v[e] = from_acc<T>(v[i * 8 + e]);
+            *reinterpret_cast<Vec<T, 8> *>(mine + ((i ^ (lane & 7)) << 4)) = w;   // the map's 128-byte swizzle
+        }
+        if (o.tma) {
+            send(&o.map, buf, col, row0, batch);
+            return;
+        }
+        // an empty group keeps next()'s count of stores in step
+        if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        __syncwarp();
+        T *out = o.out + batch * o.stride;
+        for (int r = 0; r < 32 && row0 + r < o.rows; ++r)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int c = h * 32 + lane;
+                if (col + c < o.cols)
+                    out[(long)(row0 + r) * o.ld + col + c] =
+                        *reinterpret_cast<const T *>(buf + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
+            }
+        __syncwarp();
+    }
+};
 
 // Shared-memory matrix descriptor, 128-byte swizzle.  K-major: rows 128 bytes apart, groups of 8 rows
 // 1024 bytes apart.  MN-major: blocks of 64 rows x 64 k (8192 bytes, the leading offset), in each the
@@ -155,9 +227,14 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t smem_addr) {
 // 16 k further on: 32 bytes along a swizzled row, or two 8-deep groups.
 template <bool MN> constexpr uint32_t k_step = (MN ? 2048u : 32u) >> 4;
 
-struct TileAt { int batch, m, n; };
+struct TileAt { int batch, m, n, half; };   // half: -1 whole tile, 0 / 1 its left / right half
 __device__ __forceinline__ TileAt tile_at(const TileGrid &g, int t) {
     TileAt r;
+    r.half = -1;
+    if (t >= g.whole) {
+        r.half = (t - g.whole) & 1;
+        t = g.whole + ((t - g.whole) >> 1);
+    }
     r.batch = t / g.per;
     int i = t - r.batch * g.per;
     if (g.triangle) {
@@ -181,14 +258,15 @@ template <int CG, int BN> struct GemmLayout {
     static constexpr int BROWS = BN / CG;                     // rows of B one CTA loads
     static constexpr int ABYTES = 128 * 128, BBYTES = BROWS * 128;
     static constexpr int STAGE = ABYTES + BBYTES;
-    static constexpr int STAGES = 200 * 1024 / STAGE < 8 ? 200 * 1024 / STAGE : 8;
-    static constexpr int SMEM = STAGES * STAGE + 1024 + 256;
+    static constexpr int STAGES = 192 * 1024 / STAGE < 8 ? 192 * 1024 / STAGE : 8;
+    static constexpr int STAGING = 4 * 2 * 4096;              // two buffers for each epilogue warp
+    static constexpr int SMEM = STAGES * STAGE + STAGING + 1024 + 256;
     static constexpr int TMEM_COLS = 2 * BN;
 };
 
 // Epi: { using Params; static constexpr bool kTwoMaps (B's rows come half from map 0, half from map 1);
-//        static void store(const Params &, TileAt, int row, uint32_t tmem) } -- called by all 128 epilogue threads,
-// `row` = global row of the thread's accumulator row, `tmem` = address of its first column.
+//        static void store<BN>(const Params &, TileAt, int row0, uint32_t tmem, Stager &) } -- called by the four
+// epilogue warps, `row0` = row of the matrix of the warp's first accumulator row, `tmem` = address of its first column.
 template <int CG, int BN, bool A_MN, bool B_MN, class Epi>
 __global__ void __launch_bounds__(G_THREADS, 1)
 tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
@@ -196,7 +274,7 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
     constexpr int ST = L::STAGES;
     extern __shared__ unsigned char smraw[];
     unsigned char *sm = (unsigned char *)(((uintptr_t)smraw + 1023) & ~(uintptr_t)1023);
-    unsigned long long *bars = (unsigned long long *)(sm + ST * L::STAGE);
+    unsigned long long *bars = (unsigned long long *)(sm + ST * L::STAGE + L::STAGING);
     // [0, 8) stage full, [8, 16) stage free, [16, 18) accumulator full, [18, 20) accumulator free
     uint32_t *tmem_slot = (uint32_t *)(bars + 20);
     volatile int *gave_up = (volatile int *)(bars + 21);
@@ -236,6 +314,9 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
     if (CG == 2) cluster_barrier();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
+    // everything above needs nothing of the kernel before this one in the stream
+    wait_for_previous_kernel();
+    let_next_kernel_start();
 
     if (warp == 0 && lane == 0) {
         // ---------------- loads ----------------
@@ -246,6 +327,10 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
             const TileAt at = tile_at(g, t);
             const int za = g.za ? at.batch : 0, zb = g.zb ? at.batch : 0;
             const int arow = at.m * (128 * CG) + (int)rank * 128;
+            // a half tile uses the first half of the rows of B that each CTA loads
+            const int shift = at.half > 0 ? 1 : 0, rows = at.half < 0 ? L::BROWS : L::BROWS / 2;
+            const int brow = Epi::kTwoMaps ? at.n * (BN / 2) + shift * (BN / 4)
+                                           : at.n * BN + shift * (BN / 2) + (int)rank * rows;
             for (int it = 0; it < iters; ++it) {
                 if (*gave_up || !mbar_wait_bounded(smem_u32(bars + 8 + s), phase)) {
                     ok = false;
@@ -263,7 +348,6 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
                     tma_tile<CG>(sa, &p.a[seg], full, k, arow, za);
                 }
                 if constexpr (Epi::kTwoMaps) {
-                    const int brow = at.n * (BN / 2);
                     if constexpr (CG == 2) {
                         tma_tile<CG>(sb, &p.b[rank], full, k, brow, zb);
                     } else {
@@ -271,12 +355,11 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
                         tma_tile<CG>(sb + BN / 2 * 128, &p.b[1], full, k, brow, zb);
                     }
                 } else if constexpr (B_MN) {
-                    const int brow = at.n * BN + (int)rank * L::BROWS;
 #pragma unroll
                     for (int i = 0; i < L::BROWS / 64; ++i)
                         tma_tile<CG>(sb + i * 8192, &p.b[seg], full, brow + i * 64, k, zb);
                 } else {
-                    tma_tile<CG>(sb, &p.b[seg], full, k, at.n * BN + (int)rank * L::BROWS, zb);
+                    tma_tile<CG>(sb, &p.b[seg], full, k, brow, zb);
                 }
                 ++fills;
                 if (++s == ST) {
@@ -306,7 +389,7 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
                 break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t d = tmem + buf * BN;
+            const uint32_t d = tmem + buf * BN, idesc = t >= g.whole ? g.idesc_half : g.idesc;
             for (int it = 0; it < iters; ++it) {
                 if (!mbar_wait_bounded(smem_u32(bars + s), phase)) {
                     ok = false;
@@ -317,7 +400,7 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
                 const uint64_t da = operand_desc<A_MN>(sa), db = operand_desc<B_MN>(sa + L::ABYTES);
 #pragma unroll
                 for (int k = 0; k < G_KB / 16; ++k)
-                    mma_f16<CG>(d, da + k * k_step<A_MN>, db + k * k_step<B_MN>, g.idesc, it > 0 || k > 0 ? 1u : 0u);
+                    mma_f16<CG>(d, da + k * k_step<A_MN>, db + k * k_step<B_MN>, idesc, it > 0 || k > 0 ? 1u : 0u);
                 mma_commit<CG>(smem_u32(bars + 8 + s));
                 if (++s == ST) {
                     s = 0;
@@ -331,6 +414,7 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
         // ---------------- epilogue ----------------
         const int quarter = warp & 3;   // the TMEM lanes this warp may read
         const uint32_t freed = CG == 2 ? map_to_rank(smem_u32(bars + 18), 0) : smem_u32(bars + 18);
+        Stager stager{sm + ST * L::STAGE + (warp - 2) * 8192, 0};
         int n = 0;
         for (int t = first; t < g.total; t += step, ++n) {
             const int buf = n & 1;
@@ -340,8 +424,8 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const TileAt at = tile_at(g, t);
-            const int row = at.m * (128 * CG) + (int)rank * 128 + quarter * 32 + lane;
-            Epi::template store<BN>(p.epi, at, row, tmem + buf * BN + ((uint32_t)(quarter * 32) << 16));
+            const int row0 = at.m * (128 * CG) + (int)rank * 128 + quarter * 32;
+            Epi::template store<BN>(p.epi, at, row0, tmem + buf * BN + ((uint32_t)(quarter * 32) << 16), stager);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) {
@@ -349,6 +433,7 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
                 else mbar_arrive(freed + buf * 8);
             }
         }
+        Stager::drain();
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -363,45 +448,23 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
     if (tid == 0 && *gave_up) atomicExch(g.err, 1);
 }
 
-// 32 consecutive values of a row, columns [col, col + 32) of which those below `cols` exist; `wide`: the
-// row starts on a 16-byte boundary.
-template <class T>
-__device__ __forceinline__ void store_row32(T *row, int col, int cols, bool wide, const float (&v)[32]) {
-    if (wide && col + 32 <= cols) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            Vec<T, 8> o;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) o.v[e] = from_acc<T>(v[i * 8 + e]);
-            store_vec<T, 8>(row + col + i * 8, o);
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 32; ++e)
-            if (col + e < cols) row[col + e] = from_acc<T>(v[e]);
-    }
-}
-
 // A plain product, rounded once: the batch index picks the output.
 template <class T>
 struct StoreEpi {
     struct Params {
-        T *out[2];
-        long ld[2];
-        int M, N;
-        bool wide;
+        Output<T> out[2];
     };
     static constexpr bool kTwoMaps = false;
     template <int BN>
-    static __device__ __forceinline__ void store(const Params &p, TileAt at, int row, uint32_t tmem) {
-        T *out = p.out[at.batch] + (long)row * p.ld[at.batch];
+    static __device__ __forceinline__ void store(const Params &p, TileAt at, int row0, uint32_t tmem, Stager &st) {
+        const Output<T> &o = p.out[at.batch];
+        const int first = at.n * BN + (at.half > 0 ? BN / 2 : 0), width = at.half < 0 ? BN : BN / 2;
+        if (row0 >= o.rows) return;
 #pragma unroll 1
-        for (int c = 0; c < BN; c += 32) {
-            const int col = at.n * BN + c;
-            if (col >= p.N) break;   // uniform over the warp
-            float v[32];
-            tmem_load32(tmem + c, v);
-            if (row < p.M) store_row32(out, col, p.N, p.wide, v);
+        for (int c = 0; c < width && first + c < o.cols; c += 64) {
+            float v[64];
+            tmem_load64(tmem + c, v);
+            st.put(o, row0, first + c, 0, v);
         }
     }
 };
@@ -413,7 +476,9 @@ inline uint32_t gemm_idesc(int cg, int bn, bool a_mn, bool b_mn, int fmt) {
     return (1u << 4) | ((uint32_t)fmt << 7) | ((uint32_t)fmt << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
            ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(128 * cg >> 4) << 24);
 }
-// A batch of row-major matrices as TMA sees it; box: 64 contiguous elements x `box_rows` rows.
+// A batch of row-major matrices as TMA sees it; box: 64 contiguous elements x `box_rows` rows.  TMA works in units of
+// 16 bytes (a store that ends inside one writes all of it), so `cols` is a multiple of 8: scratch matrices are
+// padded to one, with zeros, and are given with their padding.
 inline void gemm_map(CUtensorMap *map, const void *base, long cols, long rows, long batch, long ld, long batch_stride,
                      int box_rows, int fmt) {
     FITRE_REQUIRE(encode_fn(), FITRE_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
@@ -426,10 +491,22 @@ inline void gemm_map(CUtensorMap *map, const void *base, long cols, long rows, l
 }
 // What TMA can read in place.
 inline bool tma_readable(const void *p, long ld) { return aligned16(p) && ld % 8 == 0; }
+// An output and, where TMA can write it, its map.
+template <class T>
+Output<T> gemm_output(void *out, long cols, long rows, long batch, long ld, long stride, int fmt) {
+    Output<T> o = {};
+    o.out = (T *)out;
+    if (!out) return o;
+    o.ld = ld, o.stride = stride, o.rows = (int)rows, o.cols = (int)cols;
+    o.tma = cols % 8 == 0 && tma_readable(out, ld) && (batch == 1 || stride % 8 == 0);
+    if (o.tma) gemm_map(&o.map, out, cols, rows, batch, ld, stride, 32, fmt);
+    return o;
+}
 
+// `dependent`: the kernel before it in the stream is this library's and lets this one start its set-up early.
 template <int CG, int BN, bool A_MN, bool B_MN, class Epi>
 void gemm_launch(fitre_context *ctx, GemmArgs<typename Epi::Params> &args, int M, int N, int batch, bool triangle,
-                 long K, int nseg, int fmt, const char *name) {
+                 long K, int nseg, int fmt, const char *name, bool dependent) {
     using L = GemmLayout<CG, BN>;
     auto kernel = tile_gemm_kernel<CG, BN, A_MN, B_MN, Epi>;
     TileGrid &g = args.g;
@@ -439,29 +516,34 @@ void gemm_launch(fitre_context *ctx, GemmArgs<typename Epi::Params> &args, int M
     const long per = triangle ? (long)g.tilesM * (g.tilesM + 1) / 2 : (long)g.tilesM * g.tilesN;
     FITRE_REQUIRE(per * batch < (1l << 30), FITRE_ERR_TOO_LARGE, "too many tiles");
     g.per = (int)per;
-    g.total = (int)per * batch;
+    const int room = kLmSms / CG, tiles = (int)per * batch, left = tiles % room;
+    // (64 columns are the least an epilogue stores at a time; two maps on one SM load no half tiles)
+    g.whole = left > 0 && left <= room / 2 && !(Epi::kTwoMaps && CG == 1) ? tiles - left : tiles;
+    g.total = g.whole + 2 * (tiles - g.whole);
     g.triangle = triangle;
     g.kblocks = (int)((K + G_KB - 1) / G_KB);
     g.nseg = nseg;
     g.idesc = gemm_idesc(CG, BN, A_MN, B_MN, fmt);
+    g.idesc_half = gemm_idesc(CG, BN / 2, A_MN, B_MN, fmt);
     g.err = (int *)(ctx->dscal + 4000);
     static thread_local int ready = -1;
     if (ready != ctx->device) {
         FITRE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM));
         ready = ctx->device;
     }
-    const int room = kLmSms / CG;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((g.total < room ? g.total : room) * CG));
     cfg.blockDim = dim3(G_THREADS);
     cfg.dynamicSmemBytes = L::SMEM;
     cfg.stream = ctx->stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = CG;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = dependent ? 2 : 1;
     FITRE_CUDA(cudaLaunchKernelEx(&cfg, kernel, args));
     check_launch(ctx, name);
 }

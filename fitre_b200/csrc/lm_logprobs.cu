@@ -9,7 +9,7 @@
 // exceeds it by 10: sums of exponentials up to e^10 lose nothing in fp32, and rescaling becomes rare.
 // The sweep runs on pairs (packed fp32 arithmetic, 16-bit packed maxima): 4.5 instructions per element
 // instead of 8, which would be more than the issue slots one read of memory leaves.  An entry of
-// -inf would put 0 * -inf into t; that is noticed per vector, which is then done again with care.
+// -inf would put 0 * -inf into t; that is noticed per batch of loads, which is then done again with care.
 // The alternatives need no second sweep either: the k-th largest of the threads' maxima is a
 // lower bound of the k-th largest element, so only the vectors of the few threads whose maximum reaches
 // it are read again (from L2) and filtered into lists that each warp keeps sorted across its lanes; lists
@@ -166,32 +166,39 @@ template <class A> struct Running {
         st.s += p;
         st.t += p * d;
     }
-    template <class T, int VEC> __device__ __forceinline__ void vector(const Vec<T, VEC> &x) {
-        if constexpr (sizeof(A) == 8) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) element(to_acc<A>(x.v[e]));
-        } else {
+    // `n` whole vectors; their largest element has been followed
+    template <int n, class T, int VEC> __device__ __forceinline__ void vectors(const Vec<T, VEC> *x) {
+        bool careful = true;
+        if constexpr (sizeof(A) == 4) {
             using P = Simd<float, 2>;
             const P back = P::splat(-st.m), l2e = P::splat(1.4426950408889634f);
-            P v[VEC / 2], s = P::splat(0), t = s;
-            widen(x, v);
+            P s = P::splat(0), t = s;
 #pragma unroll
-            for (int i = 0; i < VEC / 2; ++i) {
-                const P d = add(v[i], back);
-                float a, b;
-                mul(d, l2e).split(a, b);
-                const P p = P::of(exp2_fast(a), exp2_fast(b));
-                s = add(s, p);
-                t = fma(p, d, t);
+            for (int u = 0; u < n; ++u) {
+                P v[VEC / 2];
+                widen(x[u], v);
+#pragma unroll
+                for (int i = 0; i < VEC / 2; ++i) {
+                    const P d = add(v[i], back);
+                    float a, b;
+                    mul(d, l2e).split(a, b);
+                    const P p = P::of(exp2_fast(a), exp2_fast(b));
+                    s = add(s, p);
+                    t = fma(p, d, t);
+                }
             }
             const float tt = t.sum();
-            if (tt == tt) {
+            careful = tt != tt;
+            if (!careful) {
                 st.s += s.sum();
                 st.t += tt;
-            } else {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) element(to_acc<float>(x.v[e]));
             }
+        }
+        if (careful) {
+#pragma unroll
+            for (int u = 0; u < n; ++u)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) element(to_acc<A>(x[u].v[e]));
         }
     }
 };
@@ -252,51 +259,54 @@ token_logprobs_kernel(const T *__restrict__ logits, long ld, const long long *__
     const T *xv = x + vbase;
 
     Running<A> run;
-    Vec<T, VEC> raw[L_UNROLL], next[L_UNROLL];
+    Vec<T, VEC> raw[2][L_UNROLL];
     int at = tid;
-    // whole batches, the next one's loads issued before this one's arithmetic
-    const int batches = nvec / (THREADS * L_UNROLL);
-    if (batches) {
+    auto load = [&](Vec<T, VEC> (&to)[L_UNROLL], int from) {
 #pragma unroll
-        for (int u = 0; u < L_UNROLL; ++u) raw[u] = load_vec<T, VEC>(xv + (long)(at + u * THREADS) * VEC);
-    }
-    for (int b = 0; b < batches; ++b) {
-        at += THREADS * L_UNROLL;
-        if (b + 1 < batches) {
+        for (int u = 0; u < L_UNROLL; ++u) to[u] = load_vec<T, VEC>(xv + (long)(from + u * THREADS) * VEC);
+    };
+    auto use = [&](const Vec<T, VEC> (&of)[L_UNROLL]) {
+        A m = vec_max(of[0]);
 #pragma unroll
-            for (int u = 0; u < L_UNROLL; ++u) next[u] = load_vec<T, VEC>(xv + (long)(at + u * THREADS) * VEC);
-        }
-        A m = vec_max(raw[0]);
-#pragma unroll
-        for (int u = 1; u < L_UNROLL; ++u) m = N::max(m, vec_max(raw[u]));
+        for (int u = 1; u < L_UNROLL; ++u) m = N::max(m, vec_max(of[u]));
         run.follow(m);
-#pragma unroll
-        for (int u = 0; u < L_UNROLL; ++u) run.vector(raw[u]);
-#pragma unroll
-        for (int u = 0; u < L_UNROLL; ++u) raw[u] = next[u];
+        run.template vectors<L_UNROLL>(of);
+    };
+    // whole batches, each one's loads issued before the arithmetic of the one before it
+    const int batches = nvec / (THREADS * L_UNROLL);
+    constexpr int STEP = THREADS * L_UNROLL;
+    if (batches) load(raw[0], at);
+    for (int b = 0; b < batches; b += 2) {
+        if (b + 1 < batches) load(raw[1], at + STEP);
+        use(raw[0]);
+        if (b + 1 < batches) {
+            if (b + 2 < batches) load(raw[0], at + 2 * STEP);
+            use(raw[1]);
+        }
+        at += 2 * STEP;
     }
+    at = tid + batches * STEP;
 #pragma unroll
     for (int u = 0; u < L_UNROLL; ++u)
-        if (at + u * THREADS < nvec) raw[u] = load_vec<T, VEC>(xv + (long)(at + u * THREADS) * VEC);
+        if (at + u * THREADS < nvec) raw[0][u] = load_vec<T, VEC>(xv + (long)(at + u * THREADS) * VEC);
 #pragma unroll
     for (int u = 0; u < L_UNROLL; ++u)
         if (at + u * THREADS < nvec) {
-            run.follow(vec_max(raw[u]));
-            run.vector(raw[u]);
+            run.follow(vec_max(raw[0][u]));
+            run.template vectors<1>(&raw[0][u]);
         }
     if (tid < edges) {
         const A v = to_acc<A>(x[tid < head ? lo + tid : tail0 + (tid - head)]);
         run.follow(v);
         run.element(v);
     }
-    Stats<A> st = run.st;
+    // the warp's statistics: all lanes onto the largest reference, then plain sums
+    Stats<A> st{warp_max(run.st.m), 0, 0};
+    st = join(st, run.st);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        Stats<A> other;
-        other.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-        other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-        other.t = __shfl_xor_sync(0xffffffffu, st.t, o);
-        st = (lane & o) ? join(other, st) : join(st, other);
+        st.s += __shfl_xor_sync(0xffffffffu, st.s, o);
+        st.t += __shfl_xor_sync(0xffffffffu, st.t, o);
     }
     if (lane == 0) wstat[warp] = st;
     if (TOP) {
@@ -339,11 +349,13 @@ token_logprobs_kernel(const T *__restrict__ logits, long ld, const long long *__
                 const bool in = vec < nvec;
                 Vec<T, VEC> raw;
                 if (in) raw = load_vec<T, VEC>(xv + (long)vec * VEC);
+                const bool worth = in && (vec_max(raw) >= bound || bound == -N::inf());
+                if (__any_sync(0xffffffffu, worth))
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
-                    A v = in ? to_acc<A>(raw.v[e]) : -N::inf();
+                    A v = worth ? to_acc<A>(raw.v[e]) : -N::inf();
                     if (v != v) v = -N::inf();
-                    use(in && v >= bound, v, vbase + vec * VEC + e);
+                    use(worth && v >= bound, v, vbase + vec * VEC + e);
                 }
             }
         };

@@ -112,32 +112,53 @@ template <class T, int VEC, int G, int CH> struct RowPart {
             }
         return q.sum();
     }
-    // y = v r gamma + beta, `gamma`, `beta` and `y` at this thread's first element
-    template <class W> __device__ __forceinline__ void store(A r, const W *gamma, const W *beta, T *y) const {
+    // y = v r gamma + beta, `gamma`, `beta` and `y` at this thread's first element.  AFFINE: both are there.
+    // Their loads go out together, four chunks at a time: one after the other they would cost an L1 latency each.
+    template <bool AFFINE, class W>
+    __device__ __forceinline__ void store(A r, const W *gamma, const W *beta, T *y) const {
         const P scale = P::splat(r);
+        constexpr int BATCH = CH < 4 ? CH : 4;
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
-            if (has(c)) {
-                P o[PV], w[PV];
+        for (int c0 = 0; c0 < CH; c0 += BATCH) {
+            Vec<W, VEC> gm[BATCH], bt[BATCH];
+            if (AFFINE) {
 #pragma unroll
-                for (int i = 0; i < PV; ++i) o[i] = mul(v[c][i], scale);
-                if (gamma) {
-                    widen(load_vec<W, VEC>(gamma + c * G * VEC), w);
-#pragma unroll
-                    for (int i = 0; i < PV; ++i) o[i] = mul(o[i], w[i]);
-                }
-                if (beta) {
-                    widen(load_vec<W, VEC>(beta + c * G * VEC), w);
-#pragma unroll
-                    for (int i = 0; i < PV; ++i) o[i] = add(o[i], w[i]);
-                }
-                store_vec<T, VEC>(y + c * G * VEC, narrowed<T, VEC>(o));
+                for (int c = 0; c < BATCH; ++c)
+                    if (has(c0 + c)) {
+                        gm[c] = load_vec<W, VEC>(gamma + (c0 + c) * G * VEC);
+                        bt[c] = load_vec<W, VEC>(beta + (c0 + c) * G * VEC);
+                    }
             }
+#pragma unroll
+            for (int c = 0; c < BATCH; ++c) {
+                P o[PV], w[PV], u[PV];
+#pragma unroll
+                for (int i = 0; i < PV; ++i) o[i] = mul(v[c0 + c][i], scale);
+                if (AFFINE) {
+                    widen(gm[c], w);
+                    widen(bt[c], u);
+#pragma unroll
+                    for (int i = 0; i < PV; ++i) o[i] = fma(o[i], w[i], u[i]);
+                } else if (has(c0 + c)) {
+                    if (gamma) {
+                        widen(load_vec<W, VEC>(gamma + (c0 + c) * G * VEC), w);
+#pragma unroll
+                        for (int i = 0; i < PV; ++i) o[i] = mul(o[i], w[i]);
+                    }
+                    if (beta) {
+                        widen(load_vec<W, VEC>(beta + (c0 + c) * G * VEC), u);
+#pragma unroll
+                        for (int i = 0; i < PV; ++i) o[i] = add(o[i], u[i]);
+                    }
+                }
+                if (has(c0 + c)) store_vec<T, VEC>(y + (c0 + c) * G * VEC, narrowed<T, VEC>(o));
+            }
+        }
     }
 };
 
 // Blocks that stay resident, G threads per row, the next row's elements loaded one row ahead.
-template <class T, class W, int VEC, int G>
+template <class T, class W, int VEC, int G, bool AFFINE>
 __global__ void __launch_bounds__(G, (sizeof(T) == 8 ? 512 : 1024) / G > 0 ? (sizeof(T) == 8 ? 512 : 1024) / G : 1)
 layer_norm_kernel(const T *x, long ldx, const W *__restrict__ gamma, const W *__restrict__ beta, T *y, long ldy,
                   acc_t<T> *mean, acc_t<T> *rstd, long rows, int cols, double eps) {
@@ -145,6 +166,7 @@ layer_norm_kernel(const T *x, long ldx, const W *__restrict__ gamma, const W *__
     constexpr int CH = N_ELEMS / VEC;
     __shared__ A buf[4 * (G / 32)];
     const int t = threadIdx.x;
+    const A over = A(1) / (A)cols;
     int slot = 0;
     x += t * VEC;
     y += t * VEC;
@@ -167,24 +189,24 @@ layer_norm_kernel(const T *x, long ldx, const W *__restrict__ gamma, const W *__
             for (int c = 0; c < CH; ++c)
                 if (part.has(c)) next[c] = load_vec<T, VEC>(x + after * ldx + c * G * VEC);
         }
-        const A m = group_sum<G>(part.sum(), buf, slot) / (A)cols;
-        const A r = rsqrt_acc<A>(group_sum<G>(part.centre(m), buf, slot) / (A)cols + (A)eps);
+        const A m = group_sum<G>(part.sum(), buf, slot) * over;
+        const A r = rsqrt_acc<A>(group_sum<G>(part.centre(m), buf, slot) * over + (A)eps);
         if (t == 0) {
             if (mean) mean[row] = m;
             if (rstd) rstd[row] = r;
         }
-        part.store(r, gamma, beta, y + row * ldy);
+        part.template store<AFFINE>(r, gamma, beta, y + row * ldy);
     }
 }
 
-// A warp per row of up to 1024 elements, 32 to a lane.
+// A warp per row of up to 1024 elements, N (8, 16 or 32) to a lane.
 constexpr int N_WIDE = 32;
-template <class T, class W, int VEC>
+template <class T, class W, int VEC, int N, bool AFFINE>
 __global__ void __launch_bounds__(256, sizeof(T) == 8 ? 2 : 4)
 layer_norm_warp_kernel(const T *x, long ldx, const W *__restrict__ gamma, const W *__restrict__ beta, T *y, long ldy,
                        acc_t<T> *mean, acc_t<T> *rstd, long rows, int cols, double eps) {
     using A = acc_t<T>;
-    constexpr int CH = N_WIDE / VEC;
+    constexpr int CH = N / VEC;
     const int t = threadIdx.x & 31;
     const long row = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (row >= rows) return;
@@ -208,11 +230,11 @@ layer_norm_warp_kernel(const T *x, long ldx, const W *__restrict__ gamma, const 
         if (mean) mean[row] = m;
         if (rstd) rstd[row] = r;
     }
-    part.store(r, gamma ? gamma + t * VEC : gamma, beta ? beta + t * VEC : beta, y + row * ldy + t * VEC);
+    part.template store<AFFINE>(r, gamma ? gamma + t * VEC : gamma, beta ? beta + t * VEC : beta, y + row * ldy + t * VEC);
 }
 
 // Rows on 16-byte boundaries through a ring of `stages` rows in shared memory.
-template <class T, class W, int VEC, int G>
+template <class T, class W, int VEC, int G, bool AFFINE>
 __global__ void __launch_bounds__(G, 1024 / G)
 layer_norm_ring_kernel(const T *x, long ldx, const W *__restrict__ gamma, const W *__restrict__ beta, T *y, long ldy,
                        acc_t<T> *mean, acc_t<T> *rstd, long rows, int cols, double eps, int stages, int *err) {
@@ -223,6 +245,7 @@ layer_norm_ring_kernel(const T *x, long ldx, const W *__restrict__ gamma, const 
     __shared__ A buf[4 * (G / 32)];
     const int t = threadIdx.x;
     const long step = gridDim.x;
+    const A over = A(1) / (A)cols;
     int slot = 0;
     RowRing ring(ring_raw, bars, stages, cols * (int)sizeof(T));
     ring.init();
@@ -244,17 +267,16 @@ layer_norm_ring_kernel(const T *x, long ldx, const W *__restrict__ gamma, const 
             if (part.has(c)) part.set(c, load_vec<T, VEC>(in + c * G * VEC));
             else part.clear(c);
         }
-        ring.done_reading();
-        // the sum's barrier also says that every thread has read the stage
-        const A m = group_sum<G>(part.sum(), buf, slot) / (A)cols;
+        // the sum's barrier also says that every thread has read the stage: the sum is made of what was read
+        const A m = group_sum<G>(part.sum(), buf, slot) * over;
         if (t == 0 && row + stages * step < rows) ring.fill(ring.at, x + (row + stages * step) * ldx);
         ring.advance();
-        const A r = rsqrt_acc<A>(group_sum<G>(part.centre(m), buf, slot) / (A)cols + (A)eps);
+        const A r = rsqrt_acc<A>(group_sum<G>(part.centre(m), buf, slot) * over + (A)eps);
         if (t == 0) {
             if (mean) mean[row] = m;
             if (rstd) rstd[row] = r;
         }
-        part.store(r, gamma, beta, y + row * ldy);
+        part.template store<AFFINE>(r, gamma, beta, y + row * ldy);
     }
 }
 
@@ -298,18 +320,22 @@ template <class T, class W, int VEC, int G, int CH> struct BackPart {
     using P = SimdOf<T, VEC>;
     static constexpr int PV = VEC / kPack<VEC>;
     P dg[CH][PV], db[CH][PV], xh[CH][PV], g[CH][PV];
+    Vec<W, VEC> gm[CH];
     int left;
-    __device__ __forceinline__ BackPart(int cols, int t) : left(cols - t * VEC) {
+    __device__ __forceinline__ BackPart(int cols, int t, const W *gamma) : left(cols - t * VEC) {
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
+        for (int c = 0; c < CH; ++c) {
 #pragma unroll
             for (int i = 0; i < PV; ++i) dg[c][i] = db[c][i] = P::splat(A(0));
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) gm[c].v[e] = from_acc<W>(A(1));
+            if (gamma && has(c)) gm[c] = load_vec<W, VEC>(gamma + c * G * VEC);
+        }
     }
     __device__ __forceinline__ bool has(int c) const { return c * G * VEC < left; }
     // sums of g and g xh over this thread's elements, from functions that give chunk c of x and dy
-    template <class X, class D>
-    __device__ __forceinline__ void take(A m, A r, const W *gamma, X &&x_at, D &&d_at, A &s1, A &s2) {
-        const P scale = P::splat(r), shift = P::splat(-m);
+    template <class X, class D> __device__ __forceinline__ void take(A m, A r, X &&x_at, D &&d_at, A &s1, A &s2) {
+        const P scale = P::splat(r), shift = P::splat(-m * r);
         P a = P::splat(A(0)), b = a;
 #pragma unroll
         for (int c = 0; c < CH; ++c)
@@ -317,13 +343,13 @@ template <class T, class W, int VEC, int G, int CH> struct BackPart {
                 P d[PV], w[PV];
                 widen(x_at(c), xh[c]);
                 widen(d_at(c), d);
-                if (gamma) widen(load_vec<W, VEC>(gamma + c * G * VEC), w);
+                widen(gm[c], w);
 #pragma unroll
                 for (int i = 0; i < PV; ++i) {
-                    xh[c][i] = mul(add(xh[c][i], shift), scale);
+                    xh[c][i] = fma(xh[c][i], scale, shift);
                     dg[c][i] = fma(d[i], xh[c][i], dg[c][i]);
                     db[c][i] = add(db[c][i], d[i]);
-                    g[c][i] = gamma ? mul(d[i], w[i]) : d[i];
+                    g[c][i] = mul(d[i], w[i]);
                     a = add(a, g[c][i]);
                     b = fma(g[c][i], xh[c][i], b);
                 }
@@ -333,13 +359,13 @@ template <class T, class W, int VEC, int G, int CH> struct BackPart {
     }
     // dx = r (g - s1 - xh s2)
     __device__ __forceinline__ void store(A r, A s1, A s2, T *dx) const {
-        const P scale = P::splat(r), back1 = P::splat(-s1), back2 = P::splat(-s2);
+        const P scale = P::splat(r), back1 = P::splat(-s1 * r), back2 = P::splat(-s2 * r);
 #pragma unroll
         for (int c = 0; c < CH; ++c)
             if (has(c)) {
                 P o[PV];
 #pragma unroll
-                for (int i = 0; i < PV; ++i) o[i] = mul(fma(xh[c][i], back2, add(g[c][i], back1)), scale);
+                for (int i = 0; i < PV; ++i) o[i] = fma(xh[c][i], back2, fma(g[c][i], scale, back1));
                 store_vec<T, VEC>(dx + c * G * VEC, narrowed<T, VEC>(o));
             }
     }
@@ -373,8 +399,8 @@ layer_norm_backward_kernel(const T *dy, long lddy, const T *x, long ldx, const W
     x += t * VEC;
     dy += t * VEC;
     dx += t * VEC;
-    if (gamma) gamma += t * VEC;
-    BackPart<T, W, VEC, G, CH> part(cols, t);
+    const A over = A(1) / (A)cols;
+    BackPart<T, W, VEC, G, CH> part(cols, t, gamma ? gamma + t * VEC : gamma);
     Vec<T, VEC> nx[CH], nd[CH];
     if (row < rows) {
 #pragma unroll
@@ -387,7 +413,7 @@ layer_norm_backward_kernel(const T *dy, long lddy, const T *x, long ldx, const W
     for (; row < rows; row += step) {
         const A r = rstd[row];
         A s1, s2;
-        part.take(mean[row], r, gamma, [&](int c) { return nx[c]; }, [&](int c) { return nd[c]; }, s1, s2);
+        part.take(mean[row], r, [&](int c) { return nx[c]; }, [&](int c) { return nd[c]; }, s1, s2);
         if (row + step < rows) {
 #pragma unroll
             for (int c = 0; c < CH; ++c)
@@ -397,7 +423,7 @@ layer_norm_backward_kernel(const T *dy, long lddy, const T *x, long ldx, const W
                 }
         }
         group_sum2<G>(s1, s2, buf, slot);
-        part.store(r, s1 / (A)cols, s2 / (A)cols, dx + row * lddx);
+        part.store(r, s1 * over, s2 * over, dx + row * lddx);
     }
     if (!partial) return;
     A *pg = partial + (long)blockIdx.x * 2 * cols + t * VEC, *pb = pg + cols;
@@ -432,7 +458,7 @@ layer_norm_backward_kernel(const T *dy, long lddy, const T *x, long ldx, const W
 }
 
 template <class T, class W, int VEC, int G>
-__global__ void __launch_bounds__(G, 768 / G > 0 ? 768 / G : 1)
+__global__ void __launch_bounds__(G, 512 / G > 0 ? 512 / G : 1)
 layer_norm_backward_ring_kernel(const T *dy, long lddy, const T *x, long ldx, const W *__restrict__ gamma,
                                 const acc_t<T> *__restrict__ mean, const acc_t<T> *__restrict__ rstd, T *dx, long lddx,
                                 acc_t<T> *partial, long rows, int cols, int stages, int *err) {
@@ -452,8 +478,8 @@ layer_norm_backward_ring_kernel(const T *dy, long lddy, const T *x, long ldx, co
             if (r < rows) ring.fill2(i, x + r * ldx, dy + r * lddy);
         }
     dx += t * VEC;
-    if (gamma) gamma += t * VEC;
-    BackPart<T, W, VEC, G, CH> part(cols, t);
+    const A over = A(1) / (A)cols;
+    BackPart<T, W, VEC, G, CH> part(cols, t, gamma ? gamma + t * VEC : gamma);
     for (long row = blockIdx.x; row < rows; row += step) {
         const A m = mean[row], r = rstd[row];
         if (!ring.wait()) {
@@ -462,14 +488,13 @@ layer_norm_backward_ring_kernel(const T *dy, long lddy, const T *x, long ldx, co
         }
         const T *xs = (const T *)ring.data() + t * VEC, *ds = (const T *)(ring.data() + bytes) + t * VEC;
         A s1, s2;
-        part.take(m, r, gamma, [&](int c) { return load_vec<T, VEC>(xs + c * G * VEC); },
+        part.take(m, r, [&](int c) { return load_vec<T, VEC>(xs + c * G * VEC); },
                   [&](int c) { return load_vec<T, VEC>(ds + c * G * VEC); }, s1, s2);
-        ring.done_reading();
         group_sum2<G>(s1, s2, buf, slot);
         if (t == 0 && row + stages * step < rows)
             ring.fill2(ring.at, x + (row + stages * step) * ldx, dy + (row + stages * step) * lddy);
         ring.advance();
-        part.store(r, s1 / (A)cols, s2 / (A)cols, dx + row * lddx);
+        part.store(r, s1 * over, s2 * over, dx + row * lddx);
     }
     if (!partial) return;
     A *pg = partial + (long)blockIdx.x * 2 * cols + t * VEC;
@@ -525,6 +550,7 @@ layer_norm_backward_long_kernel(const T *dy, long lddy, const T *x, long ldx, co
 template <class W, class A>
 __global__ void __launch_bounds__(1024)
 layer_norm_reduce_kernel(const A *__restrict__ partial, int blocks, int cols, W *dgamma, W *dbeta) {
+    wait_for_previous_kernel();
     __shared__ A s[32][33];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int at = blockIdx.x * 32 + lane;   // column of [dgamma | dbeta]
@@ -554,8 +580,7 @@ int blocks_for(long rows, int g, int threads_per_sm) {
     const long room = (long)kLmSms * (threads_per_sm > threads ? threads_per_sm / threads : 1);
     return (int)(need < room ? need : room);
 }
-constexpr int kBackThreads = 512;        // resident threads per SM of the backward kernel
-constexpr int kRingThreads = 768;        // ... of its ring form
+constexpr int kBackThreads = 512;        // resident threads per SM of the backward kernels (128 registers each)
 // Stages of a ring: as many rows as fit the block's share of 200 KB, at least 2 and at most 8 (0: too wide).
 int ring_stages(int threads, int threads_per_sm, long bytes) {
     const int blocks = threads_per_sm / threads > 0 ? threads_per_sm / threads : 1;
@@ -567,8 +592,8 @@ template <class K> void allow_shared(K kernel, size_t bytes) {
 }
 constexpr int kLongSplit = 64;           // row splits of the column sums of long rows
 
-template <class T, class W, int VEC>
-void forward_as(fitre_context *ctx, const NormArgs &a) {
+template <class T, class W, int VEC, bool AFFINE>
+void forward_with(fitre_context *ctx, const NormArgs &a) {
     using A = acc_t<T>;
     const int g = group_for(a.cols);
     const T *x = (const T *)a.x;
@@ -576,8 +601,13 @@ void forward_as(fitre_context *ctx, const NormArgs &a) {
     const W *gm = (const W *)a.gamma, *bt = (const W *)a.beta;
     A *mean = (A *)a.mean, *rstd = (A *)a.rstd;
     if (a.cols <= 32 * N_WIDE) {
-        layer_norm_warp_kernel<T, W, VEC><<<(unsigned)((a.rows + 7) / 8), 256, 0, ctx->stream>>>(
-            x, a.ldx, gm, bt, y, a.ldy, mean, rstd, a.rows, a.cols, a.eps);
+#define NORM_LAUNCH(N)                                                                                        \
+    layer_norm_warp_kernel<T, W, VEC, N, AFFINE><<<(unsigned)((a.rows + 7) / 8), 256, 0, ctx->stream>>>(     \
+        x, a.ldx, gm, bt, y, a.ldy, mean, rstd, a.rows, a.cols, a.eps)
+        if (a.cols <= 256) NORM_LAUNCH(8);
+        else if (a.cols <= 512) NORM_LAUNCH(16);
+        else NORM_LAUNCH(32);
+#undef NORM_LAUNCH
         check_launch(ctx, "layer_norm_warp_kernel");
         return;
     }
@@ -587,8 +617,8 @@ void forward_as(fitre_context *ctx, const NormArgs &a) {
     if constexpr (VEC > 1) if (stages) {
         const int room = blocks_for(a.rows, g, 1024);
 #define NORM_LAUNCH(G)                                                                                       \
-    allow_shared(layer_norm_ring_kernel<T, W, VEC, G>, stages * bytes);                                      \
-    layer_norm_ring_kernel<T, W, VEC, G><<<room, G, stages * bytes, ctx->stream>>>(                          \
+    allow_shared(layer_norm_ring_kernel<T, W, VEC, G, AFFINE>, stages * bytes);                                      \
+    layer_norm_ring_kernel<T, W, VEC, G, AFFINE><<<room, G, stages * bytes, ctx->stream>>>(                          \
         x, a.ldx, gm, bt, y, a.ldy, mean, rstd, a.rows, a.cols, a.eps, stages, (int *)(ctx->dscal + 4000))
         switch (g) {
             case 128: NORM_LAUNCH(128); break;
@@ -601,7 +631,7 @@ void forward_as(fitre_context *ctx, const NormArgs &a) {
         return;
     }
 #define NORM_LAUNCH(G)                                                                                       \
-    layer_norm_kernel<T, W, VEC, G><<<blocks, G, 0, ctx->stream>>>(                          \
+    layer_norm_kernel<T, W, VEC, G, AFFINE><<<blocks, G, 0, ctx->stream>>>(                          \
         x, a.ldx, gm, bt, y, a.ldy, mean, rstd, a.rows, a.cols, a.eps)
     switch (g) {
         case 128: NORM_LAUNCH(128); break;
@@ -619,6 +649,11 @@ void forward_as(fitre_context *ctx, const NormArgs &a) {
 }
 
 template <class T, class W, int VEC>
+void forward_as(fitre_context *ctx, const NormArgs &a) {
+    a.gamma && a.beta ? forward_with<T, W, VEC, true>(ctx, a) : forward_with<T, W, VEC, false>(ctx, a);
+}
+
+template <class T, class W, int VEC>
 void backward_as(fitre_context *ctx, const NormArgs &a) {
     using A = acc_t<T>;
     const int g = group_for(a.cols);
@@ -629,9 +664,9 @@ void backward_as(fitre_context *ctx, const NormArgs &a) {
     A *partial = a.dgamma || a.dbeta ? (A *)a.scratch : nullptr;
     int blocks = blocks_for(a.rows, g ? g : 1024, kBackThreads);
     const long bytes = 2l * a.cols * sizeof(T);
-    const int stages = VEC > 1 && g > 32 ? ring_stages(g, kRingThreads, bytes) : 0;
+    const int stages = VEC > 1 && g > 32 ? ring_stages(g, kBackThreads, bytes) : 0;
     if constexpr (VEC > 1) if (stages) {
-        blocks = blocks_for(a.rows, g, kRingThreads);
+        blocks = blocks_for(a.rows, g, kBackThreads);
 #define NORM_LAUNCH(G)                                                                                       \
     allow_shared(layer_norm_backward_ring_kernel<T, W, VEC, G>, stages * bytes);                             \
     layer_norm_backward_ring_kernel<T, W, VEC, G><<<blocks, G, stages * bytes, ctx->stream>>>(               \
@@ -661,8 +696,8 @@ void backward_as(fitre_context *ctx, const NormArgs &a) {
                 layer_norm_columns_kernel<T><<<dim3((a.cols + 255) / 256, split), 256, 0, ctx->stream>>>(
                     dy, a.lddy, x, a.ldx, mean, rstd, partial, a.rows, a.cols);
                 check_launch(ctx, "layer_norm_columns_kernel");
-                layer_norm_reduce_kernel<W, A><<<(2 * a.cols + 31) / 32, 1024, 0, ctx->stream>>>(
-                    partial, split, a.cols, (W *)a.dgamma, (W *)a.dbeta);
+                launch_after(ctx->stream, layer_norm_reduce_kernel<W, A>, dim3((2 * a.cols + 31) / 32), 1024, partial, split,
+                             a.cols, (W *)a.dgamma, (W *)a.dbeta);
                 check_launch(ctx, "layer_norm_reduce_kernel");
             }
             layer_norm_backward_long_kernel<T, W><<<blocks, 1024, 0, ctx->stream>>>(dy, a.lddy, x, a.ldx, gm, mean,
@@ -675,8 +710,8 @@ void backward_as(fitre_context *ctx, const NormArgs &a) {
     check_launch(ctx, "layer_norm_backward_kernel");
     }
     if (partial) {
-        layer_norm_reduce_kernel<W, A><<<(2 * a.cols + 31) / 32, 1024, 0, ctx->stream>>>(
-            partial, blocks, a.cols, (W *)a.dgamma, (W *)a.dbeta);
+        launch_after(ctx->stream, layer_norm_reduce_kernel<W, A>, dim3((2 * a.cols + 31) / 32), 1024, partial, blocks, a.cols,
+                     (W *)a.dgamma, (W *)a.dbeta);
         check_launch(ctx, "layer_norm_reduce_kernel");
     }
 }
@@ -718,7 +753,7 @@ void norm_dispatch(fitre_context *ctx, const NormArgs &a, bool back) {
 
 long layer_norm_backward_scratch(long rows, long cols) {
     const int g = cols <= 1024 * N_ELEMS ? group_for((int)cols) : 0;
-    const long parts = g ? blocks_for(rows, g, kRingThreads) : (rows < kLongSplit ? rows : kLongSplit);
+    const long parts = g ? blocks_for(rows, g, kBackThreads) : (rows < kLongSplit ? rows : kLongSplit);
     return parts * 2 * cols * (long)sizeof(double);
 }
 void layer_norm_forward(fitre_context *ctx, const NormArgs &a) { norm_dispatch(ctx, a, false); }

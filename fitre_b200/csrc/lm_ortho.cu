@@ -39,6 +39,7 @@ __device__ __forceinline__ double block_sum(double q, double *s) {
 template <class T, int VEC>
 __global__ void __launch_bounds__(256)
 ortho_norm_kernel(const T *in, long ld, long bstride, int rows, int cols, double *partial) {
+    let_next_kernel_start();
     __shared__ double s[8];
     const T *m = in + blockIdx.y * bstride;
     double q = 0;
@@ -56,11 +57,13 @@ ortho_norm_kernel(const T *in, long ld, long bstride, int rows, int cols, double
     if (threadIdx.x == 0) partial[(long)blockIdx.y * gridDim.x + blockIdx.x] = q;
 }
 
-// The first iterate, as a pair of fp16 matrices.
+// The first iterate, as a pair of fp16 matrices; zeros in the padding of their rows.
 template <class T, int VEC>
 __global__ void __launch_bounds__(256)
 ortho_scale_kernel(const T *in, long ld, long bstride, int rows, int cols, const double *__restrict__ partial, int parts,
                    double eps, __half *hi, __half *lo, long ldo, long ostride) {
+    wait_for_previous_kernel();
+    let_next_kernel_start();
     __shared__ double s[8];
     double q = 0;
     for (int i = threadIdx.x; i < parts; i += 256) q += partial[(long)blockIdx.y * parts + i];
@@ -82,52 +85,65 @@ ortho_scale_kernel(const T *in, long ld, long bstride, int rows, int cols, const
             store_vec<__half, VEC>(hi + r * ldo + c, h);
             store_vec<__half, VEC>(lo + r * ldo + c, l);
         }
+    for (int r = blockIdx.x; r < rows; r += gridDim.x)
+        if (cols + (int)threadIdx.x < ldo) hi[r * ldo + cols + threadIdx.x] = lo[r * ldo + cols + threadIdx.x] = __float2half_rn(0.0f);
+}
+
+// 64 consecutive fp16 values of a row of a scratch matrix whose rows are padded to a multiple of 8 (what lies in the
+// padding does not matter); `left`: columns there.
+__device__ __forceinline__ void load_row64(const __half *row, int left, Vec<__half, 8> (&w)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        w[i] = Vec<__half, 8>{};
+        if (i * 8 < left) w[i] = load_vec<__half, 8>(row + i * 8);
+    }
 }
 
 // A symmetric product: tile and, off the diagonal, its mirror image.  out = kacc * acc + kin * in; with
 // `diag`, the diagonal goes there (unscaled, fp32) and zeros take its place.
 struct SymmetricEpi {
     struct Params {
-        __half *out;
+        Output<__half> out;
+        CUtensorMap mirror;   // the same matrix, box 32 columns x 64 rows, no swizzle
         const __half *in;
         float *diag;
-        long ld, stride;
-        int n;
         float kacc, kin;
     };
     static constexpr bool kTwoMaps = false;
     template <int BN>
-    static __device__ __forceinline__ void store(const Params &p, TileAt at, int row, uint32_t tmem) {
-        __half *out = p.out + at.batch * p.stride;
-        const __half *in = p.in ? p.in + at.batch * p.stride : nullptr;
+    static __device__ __forceinline__ void store(const Params &p, TileAt at, int row0, uint32_t tmem, Stager &st) {
+        const int lane = threadIdx.x & 31, row = row0 + lane, n = p.out.rows;
+        const int first = at.n * BN + (at.half > 0 ? BN / 2 : 0), width = at.half < 0 ? BN : BN / 2;
+        if (row0 >= n) return;
+        const __half *in = p.in ? p.in + at.batch * p.out.stride + (long)row * p.out.ld : nullptr;
 #pragma unroll 1
-        for (int c = 0; c < BN; c += 32) {
-            const int col = at.n * BN + c;
-            if (col >= p.n) break;
-            float v[32];
-            tmem_load32(tmem + c, v);
-            if (row < p.n) {
+        for (int c = 0; c < width && first + c < n; c += 64) {
+            const int col = first + c;
+            Vec<__half, 8> w[8];
+            if (in) load_row64(in + col, row < n ? p.out.cols - col : 0, w);
+            float v[64];
+            tmem_load64(tmem + c, v);
 #pragma unroll
-                for (int e = 0; e < 32; ++e) v[e] *= p.kacc;
-                if (in) {
+            for (int e = 0; e < 64; ++e) v[e] *= p.kacc;
+            if (in) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (col + e < p.n) v[e] += p.kin * __half2float(in[row * p.ld + col + e]);
-                }
-                if (p.diag && row >= col && row < col + 32) {
+                for (int e = 0; e < 64; ++e) v[e] += p.kin * __half2float(w[e / 8].v[e % 8]);
+            }
+            if (p.diag && row < n && row >= col && row < col + 64) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (row == col + e) {
-                            p.diag[(long)at.batch * p.n + row] = v[e] * (1 / kScale);
-                            v[e] = 0.0f;
-                        }
-                }
-                store_row32(out + row * p.ld, col, p.n, true, v);
-                if (at.m != at.n) {
+                for (int e = 0; e < 64; ++e)
+                    if (row == col + e) {
+                        p.diag[(long)at.batch * n + row] = v[e] * (1 / kScale);
+                        v[e] = 0.0f;
+                    }
+            }
+            st.put(p.out, row0, col, at.batch, v);
+            if (at.m != at.n) {
+                // transposed in shared memory: 64 rows (these columns) of 32 (these rows)
+                unsigned char *buf = st.next();
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (col + e < p.n) out[(col + e) * p.ld + row] = __float2half_rn(v[e]);
-                }
+                for (int e = 0; e < 64; ++e) *reinterpret_cast<__half *>(buf + e * 64 + lane * 2) = __float2half_rn(v[e]);
+                Stager::send(&p.mirror, buf, row0, col, at.batch);
             }
         }
     }
@@ -136,57 +152,50 @@ struct SymmetricEpi {
 // X <- a X + B X:  v = kacc * acc + kout * ((a + d) hi + (a or a + d) lo), acc = (B without its diagonal d) hi.
 // The low part takes a alone, which is what acts on directions outside the update, but for the last
 // step, where no further step amplifies them and a + d is closer for all others.
-// T = __half: v becomes the next pair (lo in place); else v is the result.
+// T = __half: v becomes the next pair (lo in place: each warp reads its part before it stores it); else v is the result.
 template <class T>
 struct IterateEpi {
     struct Params {
-        T *out;
-        const __half *hi;
-        __half *lo;
+        Output<T> out;
+        Output<__half> lo_out;
+        const __half *hi, *lo;
         const float *diag;
-        long ldo, ostride, ldx, xstride;
-        int M, N, small;
+        long ldx, xstride;
+        int cols, small;
         float kacc, kout, a;
-        bool tall, wide;
+        int tall;
     };
     static constexpr bool kTwoMaps = false;
     template <int BN>
-    static __device__ __forceinline__ void store(const Params &p, TileAt at, int row, uint32_t tmem) {
+    static __device__ __forceinline__ void store(const Params &p, TileAt at, int row0, uint32_t tmem, Stager &st) {
         constexpr bool kLast = !std::is_same<T, __half>::value;
-        T *out = p.out + at.batch * p.ostride + (long)row * p.ldo;
+        const int row = row0 + (threadIdx.x & 31);
+        const int first = at.n * BN + (at.half > 0 ? BN / 2 : 0), width = at.half < 0 ? BN : BN / 2;
+        if (row0 >= p.out.rows) return;
+        const bool live = row < p.out.rows;
         const __half *hi = p.hi + at.batch * p.xstride + (long)row * p.ldx;
-        __half *lo = p.lo + at.batch * p.xstride + (long)row * p.ldx;
+        const __half *lo = p.lo + at.batch * p.xstride + (long)row * p.ldx;
         const float *diag = p.diag + (long)at.batch * p.small;
-        const float drow = !p.tall && row < p.M ? diag[row] : 0.0f;
+        const float drow = !p.tall && live ? diag[row] : 0.0f;
 #pragma unroll 1
-        for (int c = 0; c < BN; c += 32) {
-            const int col = at.n * BN + c;
-            if (col >= p.N) break;
-            float v[32];
-            tmem_load32(tmem + c, v);
-            if (row < p.M) {
-                // columns beyond N stay inside the row's padding to a multiple of 8
+        for (int c = 0; c < width && first + c < p.out.cols; c += 64) {
+            const int col = first + c, left = p.cols - col;
+            Vec<__half, 8> h[8], l[8];
+            load_row64(hi + col, live ? left : 0, h);
+            load_row64(lo + col, live ? left : 0, l);
+            float v[64];
+            tmem_load64(tmem + c, v);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (col + i * 8 >= p.N) break;
-                    const Vec<__half, 8> h = load_vec<__half, 8>(hi + col + i * 8), l = load_vec<__half, 8>(lo + col + i * 8);
-                    Vec<__half, 8> nh, nl;
+            for (int e = 0; e < 64; ++e) {
+                const float d = p.tall ? (e < left ? diag[col + e] : 0.0f) : drow;
+                const float x = (p.a + d) * __half2float(h[e / 8].v[e % 8]) + (kLast ? p.a + d : p.a) * __half2float(l[e / 8].v[e % 8]);
+                v[e] = p.kacc * v[e] + p.kout * x;
+            }
+            st.put(p.out, row0, col, at.batch, v);
+            if constexpr (!kLast) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int j = col + i * 8 + e;
-                        const float d = p.tall ? (j < p.N ? diag[j] : 0.0f) : drow;
-                        const float x = (p.a + d) * __half2float(h.v[e]) + (kLast ? p.a + d : p.a) * __half2float(l.v[e]);
-                        const float w = p.kacc * v[i * 8 + e] + p.kout * x;
-                        v[i * 8 + e] = w;
-                        nh.v[e] = __float2half_rn(w);
-                        nl.v[e] = __float2half_rn(w - __half2float(nh.v[e]));
-                    }
-                    if (!kLast) {
-                        store_vec<__half, 8>((__half *)out + col + i * 8, nh);
-                        store_vec<__half, 8>(lo + col + i * 8, nl);
-                    }
-                }
-                if (kLast) store_row32(out, col, p.N, p.wide, v);
+                for (int e = 0; e < 64; ++e) v[e] -= __half2float(__float2half_rn(v[e]));
+                st.put(p.lo_out, row0, col, at.batch, v);
             }
         }
     }
@@ -230,35 +239,49 @@ struct Plan {
     long bytes;
 };
 
+void mirror_map(CUtensorMap *map, const __half *base, long n, long batch, long ld, long stride) {
+    cuuint64_t dims[3] = {(cuuint64_t)ld, (cuuint64_t)n, (cuuint64_t)batch};
+    cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)(batch > 1 ? stride : n * ld) * 2};
+    cuuint32_t box[3] = {32, 64, 1};
+    FITRE_REQUIRE(encode(map, base, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_DATA_TYPE_FLOAT16),
+                  FITRE_ERR_CUDA, "tensor map refused");
+}
+
 template <int CG, int BN, bool MN>
-void symmetric(fitre_context *ctx, const Plan &pl, const __half *x, long K, long rows, long cols, long ld, long stride,
+void symmetric(fitre_context *ctx, const Plan &pl, const __half *x, long K, long rows, long ld, long stride,
                __half *out, const __half *in, float *diag, float kacc, float kin) {
-    // the matrix is rows x cols in memory; MN: its columns are the product's index
+    // MN: the matrix's columns are the product's index
     GemmArgs<SymmetricEpi::Params> g = {};
-    gemm_map(&g.a[0], x, cols, rows, pl.batch, ld, stride, a_box<CG, BN, MN>, G_F16);
-    gemm_map(&g.b[0], x, cols, rows, pl.batch, ld, stride, b_box<CG, BN, MN, false>, G_F16);
+    gemm_map(&g.a[0], x, ld, rows, pl.batch, ld, stride, a_box<CG, BN, MN>, G_F16);
+    gemm_map(&g.b[0], x, ld, rows, pl.batch, ld, stride, b_box<CG, BN, MN, false>, G_F16);
     g.g.za = g.g.zb = 1;
-    g.epi = {out, in, diag, pl.lda, pl.as, pl.small, kacc, kin};
+    g.epi.out = gemm_output<__half>(out, pl.lda, pl.small, pl.batch, pl.lda, pl.as, G_F16);
+    mirror_map(&g.epi.mirror, out, pl.small, pl.batch, pl.lda, pl.as);
+    g.epi.in = in, g.epi.diag = diag, g.epi.kacc = kacc, g.epi.kin = kin;
     gemm_launch<CG, BN, MN, MN, SymmetricEpi>(ctx, g, pl.small, pl.small, pl.batch, true, K, 1, G_F16,
-                                              "ortho_symmetric_kernel");
+                                              "ortho_symmetric_kernel", true);
 }
 
 template <int CG, int BN, class T>
-void iterate(fitre_context *ctx, const Plan &pl, const __half *x, T *out, long ldo, long ostride, bool wide, float kacc,
-             float kout, float a) {
+void iterate(fitre_context *ctx, const Plan &pl, const __half *x, T *out, long ldo, long ostride, float kacc, float kout, float a) {
     GemmArgs<typename IterateEpi<T>::Params> g = {};
     g.g.za = g.g.zb = 1;
-    g.epi = {out, x, pl.lo, pl.diag, ldo, ostride, pl.ldx, pl.xs, pl.rows, pl.cols, pl.small, kacc, kout, a, pl.tall, wide};
+    constexpr int fmt = std::is_same<T, __half>::value ? G_F16 : G_BF16;
+    g.epi.out = gemm_output<T>(out, fmt == G_F16 ? pl.ldx : pl.cols, pl.rows, pl.batch, ldo, ostride, fmt);
+    g.epi.cols = pl.cols;
+    g.epi.lo_out = gemm_output<__half>(pl.lo, pl.ldx, pl.rows, pl.batch, pl.ldx, pl.xs, G_F16);
+    g.epi.hi = x, g.epi.lo = pl.lo, g.epi.diag = pl.diag, g.epi.ldx = pl.ldx, g.epi.xstride = pl.xs;
+    g.epi.small = pl.small, g.epi.kacc = kacc, g.epi.kout = kout, g.epi.a = a, g.epi.tall = pl.tall;
     if (pl.tall) {   // X B: B is symmetric, its rows serve as its columns
-        gemm_map(&g.a[0], x, pl.cols, pl.rows, pl.batch, pl.ldx, pl.xs, a_box<CG, BN, false>, G_F16);
-        gemm_map(&g.b[0], pl.B, pl.small, pl.small, pl.batch, pl.lda, pl.as, b_box<CG, BN, false, false>, G_F16);
+        gemm_map(&g.a[0], x, pl.ldx, pl.rows, pl.batch, pl.ldx, pl.xs, a_box<CG, BN, false>, G_F16);
+        gemm_map(&g.b[0], pl.B, pl.lda, pl.small, pl.batch, pl.lda, pl.as, b_box<CG, BN, false, false>, G_F16);
         gemm_launch<CG, BN, false, false, IterateEpi<T>>(ctx, g, pl.rows, pl.cols, pl.batch, false, pl.small, 1, G_F16,
-                                                         "ortho_iterate_kernel");
+                                                         "ortho_iterate_kernel", true);
     } else {
-        gemm_map(&g.a[0], pl.B, pl.small, pl.small, pl.batch, pl.lda, pl.as, a_box<CG, BN, false>, G_F16);
-        gemm_map(&g.b[0], x, pl.cols, pl.rows, pl.batch, pl.ldx, pl.xs, b_box<CG, BN, true, false>, G_F16);
+        gemm_map(&g.a[0], pl.B, pl.lda, pl.small, pl.batch, pl.lda, pl.as, a_box<CG, BN, false>, G_F16);
+        gemm_map(&g.b[0], x, pl.ldx, pl.rows, pl.batch, pl.ldx, pl.xs, b_box<CG, BN, true, false>, G_F16);
         gemm_launch<CG, BN, false, true, IterateEpi<T>>(ctx, g, pl.rows, pl.cols, pl.batch, false, pl.small, 1, G_F16,
-                                                        "ortho_iterate_kernel");
+                                                        "ortho_iterate_kernel", true);
     }
 }
 
@@ -268,8 +291,8 @@ void start_as(fitre_context *ctx, const OrthoArgs &a, const Plan &pl) {
     ortho_norm_kernel<T, VEC><<<grid, 256, 0, ctx->stream>>>((const T *)a.in, a.ldi, a.istride, pl.rows, pl.cols,
                                                              pl.partial);
     check_launch(ctx, "ortho_norm_kernel");
-    ortho_scale_kernel<T, VEC><<<grid, 256, 0, ctx->stream>>>((const T *)a.in, a.ldi, a.istride, pl.rows, pl.cols,
-                                                              pl.partial, pl.parts, a.eps, pl.x[0], pl.lo, pl.ldx, pl.xs);
+    launch_after(ctx->stream, ortho_scale_kernel<T, VEC>, grid, 256, (const T *)a.in, a.ldi, a.istride, pl.rows, pl.cols,
+                 pl.partial, pl.parts, a.eps, pl.x[0], pl.lo, pl.ldx, pl.xs);
     check_launch(ctx, "ortho_scale_kernel");
 }
 template <class T>
@@ -305,23 +328,22 @@ void orthogonalize(fitre_context *ctx, const OrthoArgs &a) {
         const float ca = (float)a.coef[0], cb = (float)a.coef[1], cc = (float)a.coef[2];
         const __half *x = pl.x[s & 1];
         if (pl.tall) {
-            big ? symmetric<2, 256, true>(ctx, pl, x, K, pl.rows, pl.cols, pl.ldx, pl.xs, pl.A, nullptr, nullptr, 1 / kScale, 0)
-                : symmetric<1, 128, true>(ctx, pl, x, K, pl.rows, pl.cols, pl.ldx, pl.xs, pl.A, nullptr, nullptr, 1 / kScale, 0);
+            big ? symmetric<2, 256, true>(ctx, pl, x, K, pl.rows, pl.ldx, pl.xs, pl.A, nullptr, nullptr, 1 / kScale, 0)
+                : symmetric<1, 128, true>(ctx, pl, x, K, pl.rows, pl.ldx, pl.xs, pl.A, nullptr, nullptr, 1 / kScale, 0);
         } else {
-            big ? symmetric<2, 256, false>(ctx, pl, x, K, pl.rows, pl.cols, pl.ldx, pl.xs, pl.A, nullptr, nullptr, 1 / kScale, 0)
-                : symmetric<1, 128, false>(ctx, pl, x, K, pl.rows, pl.cols, pl.ldx, pl.xs, pl.A, nullptr, nullptr, 1 / kScale, 0);
+            big ? symmetric<2, 256, false>(ctx, pl, x, K, pl.rows, pl.ldx, pl.xs, pl.A, nullptr, nullptr, 1 / kScale, 0)
+                : symmetric<1, 128, false>(ctx, pl, x, K, pl.rows, pl.ldx, pl.xs, pl.A, nullptr, nullptr, 1 / kScale, 0);
         }
-        big ? symmetric<2, 256, false>(ctx, pl, pl.A, pl.small, pl.small, pl.small, pl.lda, pl.as, pl.B, pl.A, pl.diag, cc / kScale, cb)
-            : symmetric<1, 128, false>(ctx, pl, pl.A, pl.small, pl.small, pl.small, pl.lda, pl.as, pl.B, pl.A, pl.diag, cc / kScale, cb);
+        big ? symmetric<2, 256, false>(ctx, pl, pl.A, pl.small, pl.small, pl.lda, pl.as, pl.B, pl.A, pl.diag, cc / kScale, cb)
+            : symmetric<1, 128, false>(ctx, pl, pl.A, pl.small, pl.small, pl.lda, pl.as, pl.B, pl.A, pl.diag, cc / kScale, cb);
         if (s + 1 < a.steps) {
             __half *out = pl.x[(s + 1) & 1];
-            bigx ? iterate<2, 256, __half>(ctx, pl, x, out, pl.ldx, pl.xs, true, 1 / kScale, 1.0f, ca)
-                 : iterate<1, 128, __half>(ctx, pl, x, out, pl.ldx, pl.xs, true, 1 / kScale, 1.0f, ca);
+            bigx ? iterate<2, 256, __half>(ctx, pl, x, out, pl.ldx, pl.xs, 1 / kScale, 1.0f, ca)
+                 : iterate<1, 128, __half>(ctx, pl, x, out, pl.ldx, pl.xs, 1 / kScale, 1.0f, ca);
         } else {
             const float f = (float)a.scale / kScale;
-            const bool wide = tma_readable(a.out, a.ldo) && a.ostride % 8 == 0;
-            bigx ? iterate<2, 256, __nv_bfloat16>(ctx, pl, x, (__nv_bfloat16 *)a.out, a.ldo, a.ostride, wide, f / kScale, f, ca)
-                 : iterate<1, 128, __nv_bfloat16>(ctx, pl, x, (__nv_bfloat16 *)a.out, a.ldo, a.ostride, wide, f / kScale, f, ca);
+            bigx ? iterate<2, 256, __nv_bfloat16>(ctx, pl, x, (__nv_bfloat16 *)a.out, a.ldo, a.ostride, f / kScale, f, ca)
+                 : iterate<1, 128, __nv_bfloat16>(ctx, pl, x, (__nv_bfloat16 *)a.out, a.ldo, a.ostride, f / kScale, f, ca);
         }
     }
 }

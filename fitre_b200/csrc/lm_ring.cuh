@@ -1,6 +1,8 @@
 // A ring of buffers in shared memory that bulk copies fill with rows of global memory (rows on 16-byte
 // boundaries, whole multiples of 16 bytes).  One thread fills, all threads of the block read; a
-// block-wide barrier between the last read of a stage and its refill is the caller's.
+// block-wide barrier between the last read of a stage and its refill is the caller's, as is that every value
+// read has been used before it: a load whose value has been used cannot be overtaken by the refill, which is
+// written through the asynchronous proxy.
 #pragma once
 
 #include "tma_util.cuh"
@@ -45,8 +47,6 @@ struct RowRing {
     // false: the bounded wait ran out
     __device__ __forceinline__ bool wait() const { return mbar_wait(smem_u32(bars + at), phase); }
     __device__ __forceinline__ const unsigned char *data() const { return base + (size_t)at * bytes; }
-    // after a thread's last read of the stage, before the block's barrier
-    __device__ __forceinline__ void done_reading() const { release_stage_reads(); }
     __device__ __forceinline__ void advance() {
         if (++at == stages) {
             at = 0;
