@@ -179,9 +179,9 @@ template <class T, int CG, int BN>
 void forward_tiles(fitre_context *ctx, const GatedArgs &a, const Operands<T> &o) {
     GemmArgs<typename GatedEpi<T>::Params> g = {};
     const int T_ = (int)a.tokens, D = (int)up8(a.width), F = (int)a.hidden;
-    gemm_map(&g.a[0], o.x, D, T_, 1, o.ldx, 0, a_box<CG, BN, false>, fmt_of<T>);
-    gemm_map(&g.b[0], o.wg, D, F, 1, o.ldwg, 0, b_box<CG, BN, false, true>, fmt_of<T>);
-    gemm_map(&g.b[1], o.wu, D, F, 1, o.ldwu, 0, b_box<CG, BN, false, true>, fmt_of<T>);
+    gemm_operand(&g.a[0], false, o.x, T_, D, 1, o.ldx, 0, fmt_of<T>);
+    gemm_operand(&g.b[0], false, o.wg, F, D, 1, o.ldwg, 0, fmt_of<T>, 64 * CG);
+    gemm_operand(&g.b[1], false, o.wu, F, D, 1, o.ldwu, 0, fmt_of<T>, 64 * CG);
     g.epi.h = gemm_output<T>(a.h, F, T_, 1, a.ldh, 0, fmt_of<T>);
     g.epi.g = gemm_output<T>(a.g, F, T_, 1, a.ldg, 0, fmt_of<T>);
     g.epi.u = gemm_output<T>(a.u, F, T_, 1, a.ldu, 0, fmt_of<T>);
@@ -230,10 +230,10 @@ template <class T, int CG, int BN>
 void input_gradient(fitre_context *ctx, const GatedArgs &a, const Operands<T> &o, const T *slopes, long ld, long half) {
     GemmArgs<typename StoreEpi<T>::Params> g = {};
     const int T_ = (int)a.tokens, D = (int)a.width, F = (int)a.hidden;
-    gemm_map(&g.a[0], slopes, ld, T_, 1, ld, 0, a_box<CG, BN, false>, fmt_of<T>);
-    gemm_map(&g.a[1], slopes + half, ld, T_, 1, ld, 0, a_box<CG, BN, false>, fmt_of<T>);
-    gemm_map(&g.b[0], o.wg, up8(D), F, 1, o.ldwg, 0, b_box<CG, BN, true, false>, fmt_of<T>);
-    gemm_map(&g.b[1], o.wu, up8(D), F, 1, o.ldwu, 0, b_box<CG, BN, true, false>, fmt_of<T>);
+    gemm_operand(&g.a[0], false, slopes, T_, ld, 1, ld, 0, fmt_of<T>);
+    gemm_operand(&g.a[1], false, slopes + half, T_, ld, 1, ld, 0, fmt_of<T>);
+    gemm_operand(&g.b[0], true, o.wg, up8(D), F, 1, o.ldwg, 0, fmt_of<T>);
+    gemm_operand(&g.b[1], true, o.wu, up8(D), F, 1, o.ldwu, 0, fmt_of<T>);
     g.epi.out[0] = gemm_output<T>(a.dx, D, T_, 1, a.lddx, 0, fmt_of<T>);
     gemm_launch<CG, BN, false, true, StoreEpi<T>>(ctx, g, T_, D, 1, false, F, 2, fmt_of<T>, "gated_input_gradient_kernel",
                                                     a.width % 8 == 0);
@@ -242,8 +242,8 @@ template <class T, int CG, int BN>
 void weight_gradient(fitre_context *ctx, const GatedArgs &a, const Operands<T> &o, const T *slopes, long ld, long half) {
     GemmArgs<typename StoreEpi<T>::Params> g = {};
     const int T_ = (int)a.tokens, D = (int)a.width, F = (int)a.hidden;
-    gemm_map(&g.a[0], slopes, ld, T_, 2, ld, half, a_box<CG, BN, true>, fmt_of<T>);
-    gemm_map(&g.b[0], o.x, up8(D), T_, 1, o.ldx, 0, b_box<CG, BN, true, false>, fmt_of<T>);
+    gemm_operand(&g.a[0], true, slopes, ld, T_, 2, ld, half, fmt_of<T>);
+    gemm_operand(&g.b[0], true, o.x, up8(D), T_, 1, o.ldx, 0, fmt_of<T>);
     g.g.za = 1;
     g.epi.out[0] = gemm_output<T>(a.dwg, D, F, 1, a.lddwg, 0, fmt_of<T>);
     g.epi.out[1] = gemm_output<T>(a.dwu, D, F, 1, a.lddwu, 0, fmt_of<T>);

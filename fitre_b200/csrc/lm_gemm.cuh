@@ -4,9 +4,12 @@
 // Either operand may be stored with k contiguous ("K-major") or with its row index contiguous
 // ("MN-major": A' or B' in memory); both land in shared memory through tiled TMA in the 128-byte
 // swizzle that the tensor core reads, and whatever lies outside a matrix arrives as zeros.
+// The loop that issues the loads is the longest chain of the kernel: a 4-D map that cuts the contiguous
+// dimension into runs of 64 fetches 128 rows x 128 k with one instruction per operand (against two to
+// four smaller ones, 600 -> 552 us for 4096 x 4096 x 24576); blocks at a ragged edge take smaller boxes.
 //
 // Persistent kernel, warp-specialised:
-//   warp 0     one lane issues the TMA loads of a ring of stages (64 k per stage)
+//   warp 0     one lane issues the TMA loads of a ring of stages (128 k per stage)
 //   warp 1     one lane issues tcgen05.mma; accumulators live in TMEM, two of them, so that
 //   warps 2-5  read and store one tile (Epi) while the next is being computed.  Each warp gathers 32 rows x 64
 //              columns in shared memory and sends them off as one TMA store: full cache lines, edges clipped.
@@ -23,7 +26,7 @@ namespace fitre {
 namespace {
 
 constexpr int G_THREADS = 192;
-constexpr int G_KB = 64;   // k per stage: 128 bytes, one swizzle row
+constexpr int G_KB = 128;   // k per stage: two swizzle rows of 128 bytes
 
 // Which tiles there are and where their operands come from.
 struct TileGrid {
@@ -38,9 +41,15 @@ struct TileGrid {
     int *err;
 };
 
+// An operand as the loads see it.  big: runs of 64 elements as a dimension of their own, box 64 x 128 x 2 runs,
+// for blocks of 128 elements that end at or before `lim`; edge: box 64 x 128 rows (two loads per block).
+struct alignas(64) Operand {
+    CUtensorMap big, edge;
+    int lim;
+};
 template <class P>
 struct alignas(64) GemmArgs {
-    CUtensorMap a[2], b[2];
+    Operand a[2], b[2];
     TileGrid g;
     P epi;
 };
@@ -96,6 +105,32 @@ __device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap *map, u
             : "memory");
 }
 template <int CG>
+__device__ __forceinline__ void tma_runs(uint32_t dst, const CUtensorMap *map, uint32_t bar, int y, int run, int w) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+            "[%0], [%1, {%3, %4, %5, %6}], [%2];"
+            ::"r"(dst), "l"(map), "r"(bar), "r"(0), "r"(y), "r"(run), "r"(w)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+            "[%0], [%1, {%3, %4, %5, %6}], [%2];"
+            ::"r"(dst), "l"(map), "r"(bar), "r"(0), "r"(y), "r"(run), "r"(w)
+            : "memory");
+}
+// 128 rows x 128 k of an operand, 32 KB: its contiguous dimension is k, or (MN) its rows.
+template <int CG, bool MN>
+__device__ __forceinline__ void load_operand(uint32_t dst, const Operand &o, uint32_t bar, int row, int k, int z) {
+    const int run = MN ? row : k, across = MN ? k : row;   // along and across the contiguous dimension
+    if (run + 128 <= o.lim) {
+        tma_runs<CG>(dst, &o.big, bar, across, run >> 6, z);
+    } else {
+        tma_tile<CG>(dst, &o.edge, bar, run, across, z);
+        tma_tile<CG>(dst + 16384, &o.edge, bar, run + 64, across, z);
+    }
+}
+template <int CG>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     if constexpr (CG == 2)
         asm volatile(
@@ -146,6 +181,14 @@ __device__ __forceinline__ void tmem_load64(uint32_t addr, float (&v)[64]) {
     for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// v += k * the accumulator's 64 columns
+__device__ __forceinline__ void tmem_accumulate64(uint32_t addr, float k, float (&v)[64]) {
+    float t[64];
+    tmem_load64(addr, t);
+#pragma unroll
+    for (int i = 0; i < 64; ++i) v[i] += k * t[i];
+}
+
 // Where a product's result goes: `map` for TMA stores (box 64 columns x 32 rows) where TMA can write it, else
 // `out` directly.
 template <class T> struct Output {
@@ -154,6 +197,7 @@ template <class T> struct Output {
     long ld, stride;  // elements between rows, between matrices of a batch
     int rows, cols;
     int tma;
+    int passing;      // larger than L2 can keep: its lines are the first to go
 };
 
 // An epilogue warp's two staging buffers of 32 rows x 128 bytes.
@@ -167,18 +211,51 @@ struct Stager {
         turn ^= 1;
         return base + turn * 4096;
     }
-    __device__ __forceinline__ static void send(const CUtensorMap *map, const unsigned char *buf, int x, int y, int z) {
+    __device__ __forceinline__ static void send(const CUtensorMap *map, const unsigned char *buf, int x, int y, int z, bool passing) {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if ((threadIdx.x & 31) == 0) {
-            asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map),
-                         "r"(smem_u32(buf)), "r"(x), "r"(y), "r"(z)
-                         : "memory");
+            if (passing) {
+                uint64_t policy;
+                asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+                asm volatile(
+                    "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group.L2::cache_hint [%0, {%2, %3, %4}], [%1], %5;" ::"l"(map),
+                    "r"(smem_u32(buf)), "r"(x), "r"(y), "r"(z), "l"(policy)
+                    : "memory");
+            } else {
+                asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map),
+                             "r"(smem_u32(buf)), "r"(x), "r"(y), "r"(z)
+                             : "memory");
+            }
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
     }
     __device__ __forceinline__ static void drain() {
         if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+    // A 32 x 64 block of a row-major matrix of 16-bit elements (rows on 16-byte boundaries, `left` columns and `rows`
+    // rows there, columns rounded up to 8) in a warp's registers: lane l holds the 16 bytes l % 8 of rows l / 8 + 4 i ...
+    template <class T>
+    __device__ __forceinline__ static void fetch(const T *at, long ld, int rows, int left, Vec<T, 8> (&w)[8]) {
+        const int lane = threadIdx.x & 31, c = (lane & 7) * 8, r = lane >> 3;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            w[i] = Vec<T, 8>{};
+            if (c < left && r + i * 4 < rows) w[i] = load_vec<T, 8>(at + (r + i * 4) * ld + c);
+        }
+    }
+    // ... and from there, through the next buffer, with row l in lane l.
+    template <class T> __device__ __forceinline__ void turn_rows(Vec<T, 8> (&w)[8]) {
+        const int lane = threadIdx.x & 31, u = lane & 7, r = lane >> 3;
+        unsigned char *buf = next();
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<Vec<T, 8> *>(buf + (r + i * 4) * 128 + ((u ^ ((r + i * 4) & 7)) << 4)) = w[i];
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = *reinterpret_cast<const Vec<T, 8> *>(buf + lane * 128 + ((i ^ u) << 4));
+        if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");   // in step with next()
+        __syncwarp();
     }
     // Stores 64 values of each lane's row: columns [col, col + 64), rows [row0, row0 + 32).
     template <class T> __device__ __forceinline__ void put(const Output<T> &o, int row0, int col, int batch, const float (&v)[64]) {
@@ -192,7 +269,7 @@ struct Stager {
             *reinterpret_cast<Vec<T, 8> *>(mine + ((i ^ (lane & 7)) << 4)) = w;   // the map's 128-byte swizzle
         }
         if (o.tma) {
-            send(&o.map, buf, col, row0, batch);
+            send(&o.map, buf, col, row0, batch, o.passing);
             return;
         }
         // an empty group keeps next()'s count of stores in step
@@ -212,20 +289,23 @@ struct Stager {
 };
 
 // Shared-memory matrix descriptor, 128-byte swizzle.  K-major: rows 128 bytes apart, groups of 8 rows
-// 1024 bytes apart.  MN-major: blocks of 64 rows x 64 k (8192 bytes, the leading offset), in each the
-// 8-deep groups of k 1024 bytes apart.
+// 1024 bytes apart (64 k; the next 64 are a block of their own).  MN-major: blocks of 64 rows x 128 k (16384
+// bytes, the leading offset), in each the 8-deep groups of k 1024 bytes apart.
 template <bool MN>
 __device__ __forceinline__ uint64_t operand_desc(uint32_t smem_addr) {
     uint64_t d = 0;
     d |= (uint64_t)((smem_addr & 0x3FFFF) >> 4);
-    d |= (uint64_t)(MN ? (8192 >> 4) : 1) << 16;
+    d |= (uint64_t)(MN ? (16384 >> 4) : 1) << 16;
     d |= (uint64_t)(1024 >> 4) << 32;
     d |= (uint64_t)1 << 46;
     d |= (uint64_t)2 << 61;
     return d;
 }
-// 16 k further on: 32 bytes along a swizzled row, or two 8-deep groups.
-template <bool MN> constexpr uint32_t k_step = (MN ? 2048u : 32u) >> 4;
+// The descriptor's step to the i-th group of 16 k: 32 bytes along a swizzled row and, after 64 k, the next block; or
+// two 8-deep groups.
+template <bool MN> __device__ __forceinline__ uint32_t k_step(int i, int block_bytes) {
+    return MN ? (uint32_t)(i * 2048) >> 4 : (uint32_t)((i >> 2) * block_bytes + (i & 3) * 32) >> 4;
+}
 
 struct TileAt { int batch, m, n, half; };   // half: -1 whole tile, 0 / 1 its left / right half
 __device__ __forceinline__ TileAt tile_at(const TileGrid &g, int t) {
@@ -244,10 +324,11 @@ __device__ __forceinline__ TileAt tile_at(const TileGrid &g, int t) {
         r.m = row;
         r.n = i - row * (row + 1) / 2;
     } else {
-        // bands of 8 tile rows, column by column: the tiles in flight share operands in L2
-        const int band = i / (8 * g.tilesN), first = band * 8;
-        const int high = min(8, g.tilesM - first);
-        i -= band * 8 * g.tilesN;
+        // bands of 16 tile rows, column by column: the tiles in flight share operands in L2 (bands of 8 and 32 took
+        // 1.01 and 1.05 times as long for 8192 x 24576 x 4096)
+        const int band = i / (16 * g.tilesN), first = band * 16;
+        const int high = min(16, g.tilesM - first);
+        i -= band * 16 * g.tilesN;
         r.m = first + i % high;
         r.n = i / high;
     }
@@ -256,9 +337,10 @@ __device__ __forceinline__ TileAt tile_at(const TileGrid &g, int t) {
 
 template <int CG, int BN> struct GemmLayout {
     static constexpr int BROWS = BN / CG;                     // rows of B one CTA loads
-    static constexpr int ABYTES = 128 * 128, BBYTES = BROWS * 128;
+    static_assert(BROWS == 128, "a stage holds 128 rows of either operand");
+    static constexpr int ABYTES = 128 * G_KB * 2, BBYTES = BROWS * G_KB * 2;
     static constexpr int STAGE = ABYTES + BBYTES;
-    static constexpr int STAGES = 192 * 1024 / STAGE < 8 ? 192 * 1024 / STAGE : 8;
+    static constexpr int STAGES = 3;
     static constexpr int STAGING = 4 * 2 * 4096;              // two buffers for each epilogue warp
     static constexpr int SMEM = STAGES * STAGE + STAGING + 1024 + 256;
     static constexpr int TMEM_COLS = 2 * BN;
@@ -323,6 +405,9 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
         int s = 0, fills = 0;
         uint32_t phase = 1;   // of the free barriers: a fresh barrier passes a wait for the phase before its first
         bool ok = true;
+        const uint32_t full0 = smem_u32(bars), free0 = smem_u32(bars + 8), data0 = smem_u32(sm);
+        const uint32_t land0 = CG == 2 ? map_to_rank(full0, 0) : full0;   // both CTAs' loads count on the even one's
+        const int kblocks = g.kblocks, nseg = g.nseg;
         for (int t = first; ok && t < g.total; t += step) {
             const TileAt at = tile_at(g, t);
             const int za = g.za ? at.batch : 0, zb = g.zb ? at.batch : 0;
@@ -331,40 +416,31 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
             const int shift = at.half > 0 ? 1 : 0, rows = at.half < 0 ? L::BROWS : L::BROWS / 2;
             const int brow = Epi::kTwoMaps ? at.n * (BN / 2) + shift * (BN / 4)
                                            : at.n * BN + shift * (BN / 2) + (int)rank * rows;
-            for (int it = 0; it < iters; ++it) {
-                if (*gave_up || !mbar_wait_bounded(smem_u32(bars + 8 + s), phase)) {
-                    ok = false;
-                    break;
-                }
-                const int seg = it / g.kblocks, k = (it - seg * g.kblocks) * G_KB;
-                const uint32_t sa = smem_u32(sm + s * L::STAGE), sb = sa + L::ABYTES;
-                uint32_t full = smem_u32(bars + s);
-                if (rank == 0) mbar_expect_tx(full, CG * L::STAGE);
-                if (CG == 2) full = map_to_rank(full, 0);
-                if constexpr (A_MN) {
-                    tma_tile<CG>(sa, &p.a[seg], full, arow, k, za);
-                    tma_tile<CG>(sa + 8192, &p.a[seg], full, arow + 64, k, za);
-                } else {
-                    tma_tile<CG>(sa, &p.a[seg], full, k, arow, za);
-                }
-                if constexpr (Epi::kTwoMaps) {
-                    if constexpr (CG == 2) {
-                        tma_tile<CG>(sb, &p.b[rank], full, k, brow, zb);
-                    } else {
-                        tma_tile<CG>(sb, &p.b[0], full, k, brow, zb);
-                        tma_tile<CG>(sb + BN / 2 * 128, &p.b[1], full, k, brow, zb);
+            for (int seg = 0; ok && seg < nseg; ++seg) {
+                const Operand &oa = p.a[seg], &ob = p.b[Epi::kTwoMaps ? (int)rank : seg];
+                for (int kb = 0, k = 0; kb < kblocks; ++kb, k += G_KB) {
+                    if (!mbar_wait_bounded(free0 + s * 8, phase)) {
+                        ok = false;
+                        break;
                     }
-                } else if constexpr (B_MN) {
+                    const uint32_t sa = data0 + s * L::STAGE, sb = sa + L::ABYTES, full = land0 + s * 8;
+                    if (rank == 0) mbar_expect_tx(full0 + s * 8, CG * L::STAGE);
+                    load_operand<CG, A_MN>(sa, oa, full, arow, k, za);
+                    if constexpr (Epi::kTwoMaps && CG == 1) {
+                        // gate and up rows side by side in each half of k
 #pragma unroll
-                    for (int i = 0; i < L::BROWS / 64; ++i)
-                        tma_tile<CG>(sb + i * 8192, &p.b[seg], full, brow + i * 64, k, zb);
-                } else {
-                    tma_tile<CG>(sb, &p.b[seg], full, k, brow, zb);
-                }
-                ++fills;
-                if (++s == ST) {
-                    s = 0;
-                    phase ^= 1;
+                        for (int h = 0; h < 2; ++h) {
+                            tma_tile<CG>(sb + h * 16384, &p.b[0].edge, full, k + h * 64, brow, zb);
+                            tma_tile<CG>(sb + h * 16384 + 8192, &p.b[1].edge, full, k + h * 64, brow, zb);
+                        }
+                    } else {
+                        load_operand<CG, B_MN>(sb, ob, full, brow, k, zb);
+                    }
+                    ++fills;
+                    if (++s == ST) {
+                        s = 0;
+                        phase ^= 1;
+                    }
                 }
             }
         }
@@ -384,7 +460,7 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
         bool ok = true;
         for (int t = first; ok && t < g.total; t += step, ++n) {
             const int buf = n & 1;
-            if (*gave_up || !mbar_wait_bounded(smem_u32(bars + 18 + buf), (uint32_t)(((n >> 1) & 1) ^ 1))) {
+            if (!mbar_wait_bounded(smem_u32(bars + 18 + buf), (uint32_t)(((n >> 1) & 1) ^ 1))) {
                 ok = false;
                 break;
             }
@@ -400,7 +476,8 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
                 const uint64_t da = operand_desc<A_MN>(sa), db = operand_desc<B_MN>(sa + L::ABYTES);
 #pragma unroll
                 for (int k = 0; k < G_KB / 16; ++k)
-                    mma_f16<CG>(d, da + k * k_step<A_MN>, db + k * k_step<B_MN>, idesc, it > 0 || k > 0 ? 1u : 0u);
+                    mma_f16<CG>(d, da + k_step<A_MN>(k, 128 * 128), db + k_step<B_MN>(k, L::BROWS * 128), idesc,
+                                it > 0 || k > 0 ? 1u : 0u);
                 mma_commit<CG>(smem_u32(bars + 8 + s));
                 if (++s == ST) {
                     s = 0;
@@ -489,6 +566,24 @@ inline void gemm_map(CUtensorMap *map, const void *base, long cols, long rows, l
                          fmt == G_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16),
                   FITRE_ERR_CUDA, "tensor map refused");
 }
+// An operand of `rows` x `k`: a batch of matrices, row-major with the k contiguous, or (mn) stored with the rows
+// contiguous.  edge_rows: rows of the smaller box.
+inline void gemm_operand(Operand *o, bool mn, const void *base, long rows, long k, long batch, long ld, long batch_stride,
+                         int fmt, int edge_rows = 128) {
+    const long along = mn ? rows : k, across = mn ? k : rows;
+    gemm_map(&o->edge, base, along, across, batch, ld, batch_stride, edge_rows, fmt);
+    o->lim = (int)(along / 64 * 64);
+    if (o->lim < 128) {
+        o->lim = 0;
+        return;
+    }
+    cuuint64_t dims[4] = {64, (cuuint64_t)across, (cuuint64_t)(along / 64), (cuuint64_t)batch};
+    cuuint64_t strides[3] = {(cuuint64_t)ld * 2, 128, (cuuint64_t)(batch > 1 ? batch_stride : across * ld) * 2};
+    cuuint32_t box[4] = {64, 128, 2, 1};
+    FITRE_REQUIRE(encode(&o->big, base, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                         fmt == G_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16),
+                  FITRE_ERR_CUDA, "tensor map refused");
+}
 // What TMA can read in place.
 inline bool tma_readable(const void *p, long ld) { return aligned16(p) && ld % 8 == 0; }
 // An output and, where TMA can write it, its map.
@@ -499,6 +594,7 @@ Output<T> gemm_output(void *out, long cols, long rows, long batch, long ld, long
     if (!out) return o;
     o.ld = ld, o.stride = stride, o.rows = (int)rows, o.cols = (int)cols;
     o.tma = cols % 8 == 0 && tma_readable(out, ld) && (batch == 1 || stride % 8 == 0);
+    o.passing = rows * cols * batch * (long)sizeof(T) > 64l << 20;   // half of L2
     if (o.tma) gemm_map(&o.map, out, cols, rows, batch, ld, stride, 32, fmt);
     return o;
 }
@@ -547,9 +643,5 @@ void gemm_launch(fitre_context *ctx, GemmArgs<typename Epi::Params> &args, int M
     FITRE_CUDA(cudaLaunchKernelEx(&cfg, kernel, args));
     check_launch(ctx, name);
 }
-// Box rows of the operands' maps.
-template <int CG, int BN, bool A_MN> constexpr int a_box = A_MN ? 64 : 128;
-template <int CG, int BN, bool B_MN, bool TWO> constexpr int b_box = B_MN ? 64 : TWO ? BN / 2 : BN / CG;
-
 }  // namespace
 }  // namespace fitre

@@ -89,16 +89,6 @@ ortho_scale_kernel(const T *in, long ld, long bstride, int rows, int cols, const
         if (cols + (int)threadIdx.x < ldo) hi[r * ldo + cols + threadIdx.x] = lo[r * ldo + cols + threadIdx.x] = __float2half_rn(0.0f);
 }
 
-// 64 consecutive fp16 values of a row of a scratch matrix whose rows are padded to a multiple of 8 (what lies in the
-// padding does not matter); `left`: columns there.
-__device__ __forceinline__ void load_row64(const __half *row, int left, Vec<__half, 8> (&w)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        w[i] = Vec<__half, 8>{};
-        if (i * 8 < left) w[i] = load_vec<__half, 8>(row + i * 8);
-    }
-}
-
 // A symmetric product: tile and, off the diagonal, its mirror image.  out = kacc * acc + kin * in; with
 // `diag`, the diagonal goes there (unscaled, fp32) and zeros take its place.
 struct SymmetricEpi {
@@ -115,20 +105,23 @@ struct SymmetricEpi {
         const int lane = threadIdx.x & 31, row = row0 + lane, n = p.out.rows;
         const int first = at.n * BN + (at.half > 0 ? BN / 2 : 0), width = at.half < 0 ? BN : BN / 2;
         if (row0 >= n) return;
-        const __half *in = p.in ? p.in + at.batch * p.out.stride + (long)row * p.out.ld : nullptr;
+        const __half *in = p.in ? p.in + at.batch * p.out.stride + (long)row0 * p.out.ld : nullptr;
+        Vec<__half, 8> w[8];
+        if (in) Stager::fetch(in + first, p.out.ld, n - row0, p.out.cols - first, w);
 #pragma unroll 1
         for (int c = 0; c < width && first + c < n; c += 64) {
             const int col = first + c;
-            Vec<__half, 8> w[8];
-            if (in) load_row64(in + col, row < n ? p.out.cols - col : 0, w);
             float v[64];
-            tmem_load64(tmem + c, v);
-#pragma unroll
-            for (int e = 0; e < 64; ++e) v[e] *= p.kacc;
             if (in) {
+                st.turn_rows(w);
 #pragma unroll
-                for (int e = 0; e < 64; ++e) v[e] += p.kin * __half2float(w[e / 8].v[e % 8]);
+                for (int e = 0; e < 64; ++e) v[e] = p.kin * __half2float(w[e / 8].v[e % 8]);
+                Stager::fetch(in + col + 64, p.out.ld, n - row0, p.out.cols - col - 64, w);   // the next block's
+            } else {
+#pragma unroll
+                for (int e = 0; e < 64; ++e) v[e] = 0.0f;
             }
+            tmem_accumulate64(tmem + c, p.kacc, v);
             if (p.diag && row < n && row >= col && row < col + 64) {
 #pragma unroll
                 for (int e = 0; e < 64; ++e)
@@ -143,7 +136,7 @@ struct SymmetricEpi {
                 unsigned char *buf = st.next();
 #pragma unroll
                 for (int e = 0; e < 64; ++e) *reinterpret_cast<__half *>(buf + e * 64 + lane * 2) = __float2half_rn(v[e]);
-                Stager::send(&p.mirror, buf, row0, col, at.batch);
+                Stager::send(&p.mirror, buf, row0, col, at.batch, p.out.passing);
             }
         }
     }
@@ -172,25 +165,29 @@ struct IterateEpi {
         const int row = row0 + (threadIdx.x & 31);
         const int first = at.n * BN + (at.half > 0 ? BN / 2 : 0), width = at.half < 0 ? BN : BN / 2;
         if (row0 >= p.out.rows) return;
-        const bool live = row < p.out.rows;
-        const __half *hi = p.hi + at.batch * p.xstride + (long)row * p.ldx;
-        const __half *lo = p.lo + at.batch * p.xstride + (long)row * p.ldx;
+        const __half *hi = p.hi + at.batch * p.xstride + (long)row0 * p.ldx;
+        const __half *lo = p.lo + at.batch * p.xstride + (long)row0 * p.ldx;
         const float *diag = p.diag + (long)at.batch * p.small;
-        const float drow = !p.tall && live ? diag[row] : 0.0f;
+        const float drow = !p.tall && row < p.out.rows ? diag[row] : 0.0f;
+        const int rows = p.out.rows - row0;
+        Vec<__half, 8> h[8], l[8];
+        Stager::fetch(hi + first, p.ldx, rows, (int)p.ldx - first, h);
+        Stager::fetch(lo + first, p.ldx, rows, (int)p.ldx - first, l);
 #pragma unroll 1
         for (int c = 0; c < width && first + c < p.out.cols; c += 64) {
             const int col = first + c, left = p.cols - col;
-            Vec<__half, 8> h[8], l[8];
-            load_row64(hi + col, live ? left : 0, h);
-            load_row64(lo + col, live ? left : 0, l);
             float v[64];
-            tmem_load64(tmem + c, v);
+            st.turn_rows(h);
+            st.turn_rows(l);
 #pragma unroll
             for (int e = 0; e < 64; ++e) {
                 const float d = p.tall ? (e < left ? diag[col + e] : 0.0f) : drow;
-                const float x = (p.a + d) * __half2float(h[e / 8].v[e % 8]) + (kLast ? p.a + d : p.a) * __half2float(l[e / 8].v[e % 8]);
-                v[e] = p.kacc * v[e] + p.kout * x;
+                v[e] = p.kout * ((p.a + d) * __half2float(h[e / 8].v[e % 8]) + (kLast ? p.a + d : p.a) * __half2float(l[e / 8].v[e % 8]));
             }
+            // the next block's loads travel while this one is finished
+            Stager::fetch(hi + col + 64, p.ldx, rows, (int)p.ldx - col - 64, h);
+            Stager::fetch(lo + col + 64, p.ldx, rows, (int)p.ldx - col - 64, l);
+            tmem_accumulate64(tmem + c, p.kacc, v);
             st.put(p.out, row0, col, at.batch, v);
             if constexpr (!kLast) {
 #pragma unroll
@@ -252,8 +249,8 @@ void symmetric(fitre_context *ctx, const Plan &pl, const __half *x, long K, long
                __half *out, const __half *in, float *diag, float kacc, float kin) {
     // MN: the matrix's columns are the product's index
     GemmArgs<SymmetricEpi::Params> g = {};
-    gemm_map(&g.a[0], x, ld, rows, pl.batch, ld, stride, a_box<CG, BN, MN>, G_F16);
-    gemm_map(&g.b[0], x, ld, rows, pl.batch, ld, stride, b_box<CG, BN, MN, false>, G_F16);
+    gemm_operand(&g.a[0], MN, x, MN ? ld : rows, MN ? rows : ld, pl.batch, ld, stride, G_F16);
+    g.b[0] = g.a[0];
     g.g.za = g.g.zb = 1;
     g.epi.out = gemm_output<__half>(out, pl.lda, pl.small, pl.batch, pl.lda, pl.as, G_F16);
     mirror_map(&g.epi.mirror, out, pl.small, pl.batch, pl.lda, pl.as);
@@ -273,13 +270,13 @@ void iterate(fitre_context *ctx, const Plan &pl, const __half *x, T *out, long l
     g.epi.hi = x, g.epi.lo = pl.lo, g.epi.diag = pl.diag, g.epi.ldx = pl.ldx, g.epi.xstride = pl.xs;
     g.epi.small = pl.small, g.epi.kacc = kacc, g.epi.kout = kout, g.epi.a = a, g.epi.tall = pl.tall;
     if (pl.tall) {   // X B: B is symmetric, its rows serve as its columns
-        gemm_map(&g.a[0], x, pl.ldx, pl.rows, pl.batch, pl.ldx, pl.xs, a_box<CG, BN, false>, G_F16);
-        gemm_map(&g.b[0], pl.B, pl.lda, pl.small, pl.batch, pl.lda, pl.as, b_box<CG, BN, false, false>, G_F16);
+        gemm_operand(&g.a[0], false, x, pl.rows, pl.ldx, pl.batch, pl.ldx, pl.xs, G_F16);
+        gemm_operand(&g.b[0], false, pl.B, pl.small, pl.lda, pl.batch, pl.lda, pl.as, G_F16);
         gemm_launch<CG, BN, false, false, IterateEpi<T>>(ctx, g, pl.rows, pl.cols, pl.batch, false, pl.small, 1, G_F16,
                                                          "ortho_iterate_kernel", true);
     } else {
-        gemm_map(&g.a[0], pl.B, pl.lda, pl.small, pl.batch, pl.lda, pl.as, a_box<CG, BN, false>, G_F16);
-        gemm_map(&g.b[0], x, pl.ldx, pl.rows, pl.batch, pl.ldx, pl.xs, b_box<CG, BN, true, false>, G_F16);
+        gemm_operand(&g.a[0], false, pl.B, pl.small, pl.lda, pl.batch, pl.lda, pl.as, G_F16);
+        gemm_operand(&g.b[0], true, x, pl.ldx, pl.rows, pl.batch, pl.ldx, pl.xs, G_F16);
         gemm_launch<CG, BN, false, true, IterateEpi<T>>(ctx, g, pl.rows, pl.cols, pl.batch, false, pl.small, 1, G_F16,
                                                         "ortho_iterate_kernel", true);
     }
