@@ -181,14 +181,6 @@ __device__ __forceinline__ void tmem_load64(uint32_t addr, float (&v)[64]) {
     for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// v += k * the accumulator's 64 columns
-__device__ __forceinline__ void tmem_accumulate64(uint32_t addr, float k, float (&v)[64]) {
-    float t[64];
-    tmem_load64(addr, t);
-#pragma unroll
-    for (int i = 0; i < 64; ++i) v[i] += k * t[i];
-}
-
 // Where a product's result goes: `map` for TMA stores (box 64 columns x 32 rows) where TMA can write it, else
 // `out` directly.
 template <class T> struct Output {
@@ -200,73 +192,85 @@ template <class T> struct Output {
     int passing;      // larger than L2 can keep: its lines are the first to go
 };
 
-// An epilogue warp's two staging buffers of 32 rows x 128 bytes.
+__device__ __forceinline__ void st_shared16(uint32_t addr, const uint32_t (&v)[4]) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
+__device__ __forceinline__ void ld_shared16(uint32_t addr, uint32_t (&v)[4]) {
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
+}
+// Two values rounded to a pair of 16-bit elements, and back.
+template <class T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 r = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+__device__ __forceinline__ float2 unpack_half2(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
+
+// An epilogue warp's two staging buffers of 32 rows x 128 bytes (64 elements), swizzled as TMA reads and writes
+// them, and the barrier of its loads.  Shared-memory addresses; `lane` is the row a thread works on.
 struct Stager {
-    unsigned char *base;   // 1024-byte aligned
-    int turn;
-    // the next buffer, once its last store has read it
-    __device__ __forceinline__ unsigned char *next() {
-        if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+    uint32_t base, bar;
+    volatile int *gave_up;
+    int lane, turn;
+    uint32_t phase;
+    // The next of the two buffers, once its last store has read it.
+    __device__ __forceinline__ uint32_t next() {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
         __syncwarp();
         turn ^= 1;
         return base + turn * 4096;
     }
-    __device__ __forceinline__ static void send(const CUtensorMap *map, const unsigned char *buf, int x, int y, int z, bool passing) {
+    __device__ __forceinline__ uint32_t slot(uint32_t buf, int i) const { return buf + lane * 128 + ((i ^ (lane & 7)) << 4); }
+    __device__ __forceinline__ void send(const CUtensorMap *map, uint32_t buf, int x, int y, int z, bool passing) const {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if ((threadIdx.x & 31) == 0) {
+        if (lane == 0) {
             if (passing) {
                 uint64_t policy;
                 asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
                 asm volatile(
                     "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group.L2::cache_hint [%0, {%2, %3, %4}], [%1], %5;" ::"l"(map),
-                    "r"(smem_u32(buf)), "r"(x), "r"(y), "r"(z), "l"(policy)
+                    "r"(buf), "r"(x), "r"(y), "r"(z), "l"(policy)
                     : "memory");
             } else {
                 asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map),
-                             "r"(smem_u32(buf)), "r"(x), "r"(y), "r"(z)
+                             "r"(buf), "r"(x), "r"(y), "r"(z)
                              : "memory");
             }
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
     }
-    __device__ __forceinline__ static void drain() {
-        if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __device__ __forceinline__ void drain() const {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
-    // A 32 x 64 block of a row-major matrix of 16-bit elements (rows on 16-byte boundaries, `left` columns and `rows`
-    // rows there, columns rounded up to 8) in a warp's registers: lane l holds the 16 bytes l % 8 of rows l / 8 + 4 i ...
-    template <class T>
-    __device__ __forceinline__ static void fetch(const T *at, long ld, int rows, int left, Vec<T, 8> (&w)[8]) {
-        const int lane = threadIdx.x & 31, c = (lane & 7) * 8, r = lane >> 3;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            w[i] = Vec<T, 8>{};
-            if (c < left && r + i * 4 < rows) w[i] = load_vec<T, 8>(at + (r + i * 4) * ld + c);
+    // Starts loading the same 32 x 64 block of up to two matrices into the two buffers, once both are free; `b` may be
+    // NULL.  wait() before reading them.
+    __device__ __forceinline__ void load(const CUtensorMap *a, const CUtensorMap *b, int x, int y, int z) const {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // this thread's reads of the buffers come first
+        __syncwarp();
+        if (lane == 0) {
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            mbar_expect_tx(bar, b ? 8192 : 4096);
+            tma_tile<1>(base, a, bar, x, y, z);
+            if (b) tma_tile<1>(base + 4096, b, bar, x, y, z);
         }
     }
-    // ... and from there, through the next buffer, with row l in lane l.
-    template <class T> __device__ __forceinline__ void turn_rows(Vec<T, 8> (&w)[8]) {
-        const int lane = threadIdx.x & 31, u = lane & 7, r = lane >> 3;
-        unsigned char *buf = next();
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<Vec<T, 8> *>(buf + (r + i * 4) * 128 + ((u ^ ((r + i * 4) & 7)) << 4)) = w[i];
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = *reinterpret_cast<const Vec<T, 8> *>(buf + lane * 128 + ((i ^ u) << 4));
-        if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");   // in step with next()
-        __syncwarp();
+    __device__ __forceinline__ void wait() {
+        if (!mbar_wait_bounded(bar, phase)) *gave_up = 1;
+        phase ^= 1;
     }
-    // Stores 64 values of each lane's row: columns [col, col + 64), rows [row0, row0 + 32).
-    template <class T> __device__ __forceinline__ void put(const Output<T> &o, int row0, int col, int batch, const float (&v)[64]) {
-        const int lane = threadIdx.x & 31;
-        unsigned char *buf = next(), *mine = buf + lane * 128;
+    // Stores 64 packed values of each lane's row: columns [col, col + 64), rows [row0, row0 + 32).
+    template <class T>
+    __device__ __forceinline__ void put(const Output<T> &o, int row0, int col, int batch, const uint32_t (&w)[32]) {
+        const uint32_t buf = next();
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            Vec<T, 8> w;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w.v[e] = from_acc<T>(v[i * 8 + e]);
-            *reinterpret_cast<Vec<T, 8> *>(mine + ((i ^ (lane & 7)) << 4)) = w;   // the map's 128-byte swizzle
+            const uint32_t q[4] = {w[i * 4], w[i * 4 + 1], w[i * 4 + 2], w[i * 4 + 3]};
+            st_shared16(slot(buf, i), q);
         }
         if (o.tma) {
             send(&o.map, buf, col, row0, batch, o.passing);
@@ -275,16 +279,23 @@ struct Stager {
         // an empty group keeps next()'s count of stores in step
         if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         __syncwarp();
-        T *out = o.out + batch * o.stride;
+        uint16_t *out = reinterpret_cast<uint16_t *>(o.out) + batch * o.stride;
         for (int r = 0; r < 32 && row0 + r < o.rows; ++r)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int c = h * 32 + lane;
-                if (col + c < o.cols)
-                    out[(long)(row0 + r) * o.ld + col + c] =
-                        *reinterpret_cast<const T *>(buf + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
+                uint16_t v;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(buf + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2));
+                if (col + c < o.cols) out[(long)(row0 + r) * o.ld + col + c] = v;
             }
         __syncwarp();
+    }
+    template <class T>
+    __device__ __forceinline__ void put(const Output<T> &o, int row0, int col, int batch, const float (&v)[64]) {
+        uint32_t w[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+        put(o, row0, col, batch, w);
     }
 };
 
@@ -357,7 +368,7 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
     extern __shared__ unsigned char smraw[];
     unsigned char *sm = (unsigned char *)(((uintptr_t)smraw + 1023) & ~(uintptr_t)1023);
     unsigned long long *bars = (unsigned long long *)(sm + ST * L::STAGE + L::STAGING);
-    // [0, 8) stage full, [8, 16) stage free, [16, 18) accumulator full, [18, 20) accumulator free
+    // [0, 8) stage full, [8, 16) stage free, [16, 18) accumulator full, [18, 20) accumulator free, [22, 26) epilogue loads
     uint32_t *tmem_slot = (uint32_t *)(bars + 20);
     volatile int *gave_up = (volatile int *)(bars + 21);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -376,6 +387,7 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
             mbar_init(smem_u32(bars + 16 + s), 1);
             mbar_init(smem_u32(bars + 18 + s), 4 * CG);   // one arrival per epilogue warp of the pair
         }
+        for (int s = 0; s < 4; ++s) mbar_init(smem_u32(bars + 22 + s), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -491,7 +503,7 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
         // ---------------- epilogue ----------------
         const int quarter = warp & 3;   // the TMEM lanes this warp may read
         const uint32_t freed = CG == 2 ? map_to_rank(smem_u32(bars + 18), 0) : smem_u32(bars + 18);
-        Stager stager{sm + ST * L::STAGE + (warp - 2) * 8192, 0};
+        Stager stager{smem_u32(sm + ST * L::STAGE) + (warp - 2) * 8192, smem_u32(bars + 22 + (warp - 2)), gave_up, lane, 0, 0};
         int n = 0;
         for (int t = first; t < g.total; t += step, ++n) {
             const int buf = n & 1;
@@ -510,7 +522,7 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
                 else mbar_arrive(freed + buf * 8);
             }
         }
-        Stager::drain();
+        stager.drain();
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

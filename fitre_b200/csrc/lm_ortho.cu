@@ -16,6 +16,7 @@
 // Products accumulate in fp32; the result is rounded to bf16 once, and is within about half a bf16
 // rounding of the exact polynomial before that.
 #include "lm_gemm.cuh"
+#include "lm_simd.cuh"
 
 namespace fitre {
 namespace {
@@ -95,48 +96,54 @@ struct SymmetricEpi {
     struct Params {
         Output<__half> out;
         CUtensorMap mirror;   // the same matrix, box 32 columns x 64 rows, no swizzle
-        const __half *in;
+        CUtensorMap in;       // as out's map
         float *diag;
         float kacc, kin;
+        int with_in;
     };
     static constexpr bool kTwoMaps = false;
     template <int BN>
     static __device__ __forceinline__ void store(const Params &p, TileAt at, int row0, uint32_t tmem, Stager &st) {
-        const int lane = threadIdx.x & 31, row = row0 + lane, n = p.out.rows;
+        const int row = row0 + st.lane, n = p.out.rows;
         const int first = at.n * BN + (at.half > 0 ? BN / 2 : 0), width = at.half < 0 ? BN : BN / 2;
         if (row0 >= n) return;
-        const __half *in = p.in ? p.in + at.batch * p.out.stride + (long)row0 * p.out.ld : nullptr;
-        Vec<__half, 8> w[8];
-        if (in) Stager::fetch(in + first, p.out.ld, n - row0, p.out.cols - first, w);
 #pragma unroll 1
         for (int c = 0; c < width && first + c < n; c += 64) {
             const int col = first + c;
-            float v[64];
-            if (in) {
-                st.turn_rows(w);
+            if (p.with_in) st.load(&p.in, nullptr, col, row0, at.batch);
+            float acc[64];
+            tmem_load64(tmem + c, acc);
+            if (p.with_in) st.wait();
+            const int on = p.diag && row < n ? row - col : -1;   // this row's diagonal element in the block, if 0..63
+            uint32_t w[32];
 #pragma unroll
-                for (int e = 0; e < 64; ++e) v[e] = p.kin * __half2float(w[e / 8].v[e % 8]);
-                Stager::fetch(in + col + 64, p.out.ld, n - row0, p.out.cols - col - 64, w);   // the next block's
-            } else {
+            for (int i = 0; i < 8; ++i) {
+                uint32_t q[4] = {0, 0, 0, 0};
+                if (p.with_in) ld_shared16(st.slot(st.base, i), q);
 #pragma unroll
-                for (int e = 0; e < 64; ++e) v[e] = 0.0f;
-            }
-            tmem_accumulate64(tmem + c, p.kacc, v);
-            if (p.diag && row < n && row >= col && row < col + 64) {
-#pragma unroll
-                for (int e = 0; e < 64; ++e)
-                    if (row == col + e) {
-                        p.diag[(long)at.batch * n + row] = v[e] * (1 / kScale);
-                        v[e] = 0.0f;
+                for (int j = 0; j < 4; ++j) {
+                    const int e = i * 8 + j * 2;
+                    const float2 f = unpack_half2(q[j]);
+                    float x = p.kacc * acc[e] + p.kin * f.x, y = p.kacc * acc[e + 1] + p.kin * f.y;
+                    if ((on & ~1) == e) {
+                        p.diag[(long)at.batch * n + row] = (on & 1 ? y : x) * (1 / kScale);
+                        if (on & 1) y = 0.0f;
+                        else x = 0.0f;
                     }
+                    w[i * 4 + j] = pack2<__half>(x, y);
+                }
             }
-            st.put(p.out, row0, col, at.batch, v);
+            __syncwarp();
+            st.put(p.out, row0, col, at.batch, w);
             if (at.m != at.n) {
                 // transposed in shared memory: 64 rows (these columns) of 32 (these rows)
-                unsigned char *buf = st.next();
+                const uint32_t buf = st.next() + st.lane * 2;
 #pragma unroll
-                for (int e = 0; e < 64; ++e) *reinterpret_cast<__half *>(buf + e * 64 + lane * 2) = __float2half_rn(v[e]);
-                Stager::send(&p.mirror, buf, row0, col, at.batch, p.out.passing);
+                for (int e = 0; e < 32; ++e) {
+                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(buf + e * 128), "h"((uint16_t)w[e]) : "memory");
+                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(buf + e * 128 + 64), "h"((uint16_t)(w[e] >> 16)) : "memory");
+                }
+                st.send(&p.mirror, buf - st.lane * 2, row0, col, at.batch, p.out.passing);
             }
         }
     }
@@ -150,10 +157,9 @@ template <class T>
 struct IterateEpi {
     struct Params {
         Output<T> out;
-        Output<__half> lo_out;
-        const __half *hi, *lo;
+        Output<__half> lo;
+        CUtensorMap hi;
         const float *diag;
-        long ldx, xstride;
         int cols, small;
         float kacc, kout, a;
         int tall;
@@ -161,39 +167,49 @@ struct IterateEpi {
     static constexpr bool kTwoMaps = false;
     template <int BN>
     static __device__ __forceinline__ void store(const Params &p, TileAt at, int row0, uint32_t tmem, Stager &st) {
+        using P = Simd<float, 2>;
         constexpr bool kLast = !std::is_same<T, __half>::value;
-        const int row = row0 + (threadIdx.x & 31);
+        const int row = row0 + st.lane;
         const int first = at.n * BN + (at.half > 0 ? BN / 2 : 0), width = at.half < 0 ? BN : BN / 2;
         if (row0 >= p.out.rows) return;
-        const __half *hi = p.hi + at.batch * p.xstride + (long)row0 * p.ldx;
-        const __half *lo = p.lo + at.batch * p.xstride + (long)row0 * p.ldx;
         const float *diag = p.diag + (long)at.batch * p.small;
         const float drow = !p.tall && row < p.out.rows ? diag[row] : 0.0f;
-        const int rows = p.out.rows - row0;
-        Vec<__half, 8> h[8], l[8];
-        Stager::fetch(hi + first, p.ldx, rows, (int)p.ldx - first, h);
-        Stager::fetch(lo + first, p.ldx, rows, (int)p.ldx - first, l);
+        const P kacc = P::splat(p.kacc), kout = P::splat(p.kout), a = P::splat(p.a), minus = P::splat(-1.0f);
+        st.load(&p.hi, &p.lo.map, first, row0, at.batch);
 #pragma unroll 1
         for (int c = 0; c < width && first + c < p.out.cols; c += 64) {
             const int col = first + c, left = p.cols - col;
-            float v[64];
-            st.turn_rows(h);
-            st.turn_rows(l);
+            float acc[64];
+            tmem_load64(tmem + c, acc);
+            st.wait();
+            uint32_t w[32], r[32];
 #pragma unroll
-            for (int e = 0; e < 64; ++e) {
-                const float d = p.tall ? (e < left ? diag[col + e] : 0.0f) : drow;
-                v[e] = p.kout * ((p.a + d) * __half2float(h[e / 8].v[e % 8]) + (kLast ? p.a + d : p.a) * __half2float(l[e / 8].v[e % 8]));
-            }
-            // the next block's loads travel while this one is finished
-            Stager::fetch(hi + col + 64, p.ldx, rows, (int)p.ldx - col - 64, h);
-            Stager::fetch(lo + col + 64, p.ldx, rows, (int)p.ldx - col - 64, l);
-            tmem_accumulate64(tmem + c, p.kacc, v);
-            st.put(p.out, row0, col, at.batch, v);
-            if constexpr (!kLast) {
+            for (int i = 0; i < 8; ++i) {
+                uint32_t h[4], l[4];
+                ld_shared16(st.slot(st.base, i), h);
+                ld_shared16(st.slot(st.base + 4096, i), l);
 #pragma unroll
-                for (int e = 0; e < 64; ++e) v[e] -= __half2float(__float2half_rn(v[e]));
-                st.put(p.lo_out, row0, col, at.batch, v);
+                for (int j = 0; j < 4; ++j) {
+                    const int e = i * 8 + j * 2;
+                    const float2 fh = unpack_half2(h[j]), fl = unpack_half2(l[j]);
+                    P ad = P::splat(p.a + drow);
+                    if (p.tall) ad = add(a, P::of(e < left ? diag[col + e] : 0.0f, e + 1 < left ? diag[col + e + 1] : 0.0f));
+                    P x = fma(P::of(fl.x, fl.y), kLast ? ad : a, mul(P::of(fh.x, fh.y), ad));
+                    x = fma(P::of(acc[e], acc[e + 1]), kacc, mul(x, kout));
+                    float x0, x1;
+                    x.split(x0, x1);
+                    w[i * 4 + j] = pack2<T>(x0, x1);
+                    if (!kLast) {
+                        const float2 f = unpack_half2(w[i * 4 + j]);
+                        fma(P::of(f.x, f.y), minus, x).split(x0, x1);
+                        r[i * 4 + j] = pack2<__half>(x0, x1);
+                    }
+                }
             }
+            __syncwarp();
+            st.put(p.out, row0, col, at.batch, w);
+            if constexpr (!kLast) st.put(p.lo, row0, col, at.batch, r);
+            if (c + 64 < width && col + 64 < p.out.cols) st.load(&p.hi, &p.lo.map, col + 64, row0, at.batch);
         }
     }
 };
@@ -254,7 +270,8 @@ void symmetric(fitre_context *ctx, const Plan &pl, const __half *x, long K, long
     g.g.za = g.g.zb = 1;
     g.epi.out = gemm_output<__half>(out, pl.lda, pl.small, pl.batch, pl.lda, pl.as, G_F16);
     mirror_map(&g.epi.mirror, out, pl.small, pl.batch, pl.lda, pl.as);
-    g.epi.in = in, g.epi.diag = diag, g.epi.kacc = kacc, g.epi.kin = kin;
+    if (in) gemm_map(&g.epi.in, in, pl.lda, pl.small, pl.batch, pl.lda, pl.as, 32, G_F16);
+    g.epi.with_in = in != nullptr, g.epi.diag = diag, g.epi.kacc = kacc, g.epi.kin = kin;
     gemm_launch<CG, BN, MN, MN, SymmetricEpi>(ctx, g, pl.small, pl.small, pl.batch, true, K, 1, G_F16,
                                               "ortho_symmetric_kernel", true);
 }
@@ -266,9 +283,9 @@ void iterate(fitre_context *ctx, const Plan &pl, const __half *x, T *out, long l
     constexpr int fmt = std::is_same<T, __half>::value ? G_F16 : G_BF16;
     g.epi.out = gemm_output<T>(out, fmt == G_F16 ? pl.ldx : pl.cols, pl.rows, pl.batch, ldo, ostride, fmt);
     g.epi.cols = pl.cols;
-    g.epi.lo_out = gemm_output<__half>(pl.lo, pl.ldx, pl.rows, pl.batch, pl.ldx, pl.xs, G_F16);
-    g.epi.hi = x, g.epi.lo = pl.lo, g.epi.diag = pl.diag, g.epi.ldx = pl.ldx, g.epi.xstride = pl.xs;
-    g.epi.small = pl.small, g.epi.kacc = kacc, g.epi.kout = kout, g.epi.a = a, g.epi.tall = pl.tall;
+    g.epi.lo = gemm_output<__half>(pl.lo, pl.ldx, pl.rows, pl.batch, pl.ldx, pl.xs, G_F16);
+    gemm_map(&g.epi.hi, x, pl.ldx, pl.rows, pl.batch, pl.ldx, pl.xs, 32, G_F16);
+    g.epi.diag = pl.diag, g.epi.small = pl.small, g.epi.kacc = kacc, g.epi.kout = kout, g.epi.a = a, g.epi.tall = pl.tall;
     if (pl.tall) {   // X B: B is symmetric, its rows serve as its columns
         gemm_operand(&g.a[0], false, x, pl.rows, pl.ldx, pl.batch, pl.ldx, pl.xs, G_F16);
         gemm_operand(&g.b[0], false, pl.B, pl.small, pl.lda, pl.batch, pl.lda, pl.as, G_F16);
