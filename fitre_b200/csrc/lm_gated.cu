@@ -43,6 +43,7 @@ struct GatedEpi {
         int act;
     };
     static constexpr bool kTwoMaps = true;
+    template <int BN> static __device__ __forceinline__ void begin(const Params &, TileAt, int, Stager &) {}
     template <int BN>
     static __device__ __forceinline__ void store(const Params &p, TileAt at, int row0, uint32_t tmem, Stager &st) {
         // columns: the tile's gates, then as many ups

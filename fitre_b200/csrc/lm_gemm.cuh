@@ -217,6 +217,7 @@ struct Stager {
     volatile int *gave_up;
     int lane, turn;
     uint32_t phase;
+    bool loading;
     // The next of the two buffers, once its last store has read it.
     __device__ __forceinline__ uint32_t next() {
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
@@ -249,7 +250,8 @@ struct Stager {
     }
     // Starts loading the same 32 x 64 block of up to two matrices into the two buffers, once both are free; `b` may be
     // NULL.  wait() before reading them.
-    __device__ __forceinline__ void load(const CUtensorMap *a, const CUtensorMap *b, int x, int y, int z) const {
+    __device__ __forceinline__ void load(const CUtensorMap *a, const CUtensorMap *b, int x, int y, int z) {
+        loading = true;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // this thread's reads of the buffers come first
         __syncwarp();
         if (lane == 0) {
@@ -262,6 +264,11 @@ struct Stager {
     __device__ __forceinline__ void wait() {
         if (!mbar_wait_bounded(bar, phase)) *gave_up = 1;
         phase ^= 1;
+        loading = false;
+    }
+    // after a wait elsewhere ran out: a load that was started has to land before the kernel ends
+    __device__ __forceinline__ void settle() {
+        if (loading) wait();
     }
     // Stores 64 packed values of each lane's row: columns [col, col + 64), rows [row0, row0 + 32).
     template <class T>
@@ -359,7 +366,7 @@ template <int CG, int BN> struct GemmLayout {
 
 // Epi: { using Params; static constexpr bool kTwoMaps (B's rows come half from map 0, half from map 1);
 //        static void store<BN>(const Params &, TileAt, int row0, uint32_t tmem, Stager &) } -- called by the four
-// epilogue warps, `row0` = row of the matrix of the warp's first accumulator row, `tmem` = address of its first column.
+// epilogue warps once the tile is computed, and begin<BN> before (to start loads), `row0` = row of the matrix of the warp's first accumulator row, `tmem` = address of its first column.
 template <int CG, int BN, bool A_MN, bool B_MN, class Epi>
 __global__ void __launch_bounds__(G_THREADS, 1)
 tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
@@ -503,17 +510,18 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
         // ---------------- epilogue ----------------
         const int quarter = warp & 3;   // the TMEM lanes this warp may read
         const uint32_t freed = CG == 2 ? map_to_rank(smem_u32(bars + 18), 0) : smem_u32(bars + 18);
-        Stager stager{smem_u32(sm + ST * L::STAGE) + (warp - 2) * 8192, smem_u32(bars + 22 + (warp - 2)), gave_up, lane, 0, 0};
+        Stager stager{smem_u32(sm + ST * L::STAGE) + (warp - 2) * 8192, smem_u32(bars + 22 + (warp - 2)), gave_up, lane, 0, 0, false};
         int n = 0;
         for (int t = first; t < g.total; t += step, ++n) {
             const int buf = n & 1;
+            const TileAt at = tile_at(g, t);
+            const int row0 = at.m * (128 * CG) + (int)rank * 128 + quarter * 32;
+            Epi::template begin<BN>(p.epi, at, row0, stager);
             if (!mbar_wait_bounded(smem_u32(bars + 16 + buf), (uint32_t)((n >> 1) & 1))) {
                 *gave_up = 1;
                 break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const TileAt at = tile_at(g, t);
-            const int row0 = at.m * (128 * CG) + (int)rank * 128 + quarter * 32;
             Epi::template store<BN>(p.epi, at, row0, tmem + buf * BN + ((uint32_t)(quarter * 32) << 16), stager);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
@@ -523,6 +531,7 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
             }
         }
         stager.drain();
+        stager.settle();
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -544,6 +553,7 @@ struct StoreEpi {
         Output<T> out[2];
     };
     static constexpr bool kTwoMaps = false;
+    template <int BN> static __device__ __forceinline__ void begin(const Params &, TileAt, int, Stager &) {}
     template <int BN>
     static __device__ __forceinline__ void store(const Params &p, TileAt at, int row0, uint32_t tmem, Stager &st) {
         const Output<T> &o = p.out[at.batch];

@@ -102,6 +102,10 @@ struct SymmetricEpi {
         int with_in;
     };
     static constexpr bool kTwoMaps = false;
+    template <int BN> static __device__ __forceinline__ void begin(const Params &p, TileAt at, int row0, Stager &st) {
+        const int first = at.n * BN + (at.half > 0 ? BN / 2 : 0);
+        if (p.with_in && row0 < p.out.rows && first < p.out.rows) st.load(&p.in, nullptr, first, row0, at.batch);
+    }
     template <int BN>
     static __device__ __forceinline__ void store(const Params &p, TileAt at, int row0, uint32_t tmem, Stager &st) {
         const int row = row0 + st.lane, n = p.out.rows;
@@ -110,7 +114,7 @@ struct SymmetricEpi {
 #pragma unroll 1
         for (int c = 0; c < width && first + c < n; c += 64) {
             const int col = first + c;
-            if (p.with_in) st.load(&p.in, nullptr, col, row0, at.batch);
+            if (p.with_in && c > 0) st.load(&p.in, nullptr, col, row0, at.batch);
             float acc[64];
             tmem_load64(tmem + c, acc);
             if (p.with_in) st.wait();
@@ -165,6 +169,10 @@ struct IterateEpi {
         int tall;
     };
     static constexpr bool kTwoMaps = false;
+    template <int BN> static __device__ __forceinline__ void begin(const Params &p, TileAt at, int row0, Stager &st) {
+        const int first = at.n * BN + (at.half > 0 ? BN / 2 : 0);
+        if (row0 < p.out.rows && first < p.out.cols) st.load(&p.hi, &p.lo.map, first, row0, at.batch);
+    }
     template <int BN>
     static __device__ __forceinline__ void store(const Params &p, TileAt at, int row0, uint32_t tmem, Stager &st) {
         using P = Simd<float, 2>;
@@ -175,7 +183,6 @@ struct IterateEpi {
         const float *diag = p.diag + (long)at.batch * p.small;
         const float drow = !p.tall && row < p.out.rows ? diag[row] : 0.0f;
         const P kacc = P::splat(p.kacc), kout = P::splat(p.kout), a = P::splat(p.a), minus = P::splat(-1.0f);
-        st.load(&p.hi, &p.lo.map, first, row0, at.batch);
 #pragma unroll 1
         for (int c = 0; c < width && first + c < p.out.cols; c += 64) {
             const int col = first + c, left = p.cols - col;
