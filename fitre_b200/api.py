@@ -518,35 +518,39 @@ def readVector(path, n):
 # bfloat16, float16); outputs are tensors of the caller's.  Everything is queued on the context's
 # stream.  See include/fitre_b200.h for the formulas and the treatment of special values.
 
-_DTYPES = {}
+_KINDS = {}   # element type -> (code, type of the statistics next to it)
+_TYPES = {}   # names of the types the checks below need
 
 
-def _dtype_code(t):
-    if not _DTYPES:
+def _kind(t):
+    kind = _KINDS.get(t.dtype)
+    if kind is None:
         import torch
-        _DTYPES.update({torch.float64: S.DTYPE_F64, torch.float32: S.DTYPE_F32,
-                        torch.bfloat16: S.DTYPE_BF16, torch.float16: S.DTYPE_F16})
-    code = _DTYPES.get(t.dtype)
-    if code is None:
+        if not _KINDS:
+            _TYPES.update(f64=torch.float64, f32=torch.float32, i64=torch.int64, bf16=torch.bfloat16)
+            _KINDS.update({torch.float64: (S.DTYPE_F64, torch.float64), torch.float32: (S.DTYPE_F32, torch.float32),
+                           torch.bfloat16: (S.DTYPE_BF16, torch.float32), torch.float16: (S.DTYPE_F16, torch.float32)})
+            return _kind(t)
         raise FitreError(S.ERR_UNSUPPORTED, "element type %s" % t.dtype)
-    return code
+    return kind
 
 
-def _on(ctx, t, what):
-    if not t.is_cuda or t.get_device() != ctx.device:
-        raise FitreError(S.ERR_BAD_ARG, "%s must be a tensor on CUDA device %d" % (what, ctx.device))
+def _elsewhere(ctx, what):
+    return FitreError(S.ERR_BAD_ARG, "%s must be a tensor on CUDA device %d" % (what, ctx.device))
 
 
 def _matrix(ctx, t, what, shape=None, dtype=None):
     """(pointer, row stride) of a matrix argument after its checks."""
-    _on(ctx, t, what)
-    if t.dim() != 2 or (shape is not None and tuple(t.shape) != shape):
-        raise FitreError(S.ERR_BAD_ARG, "%s must have shape %s" % (what, "(rows, cols)" if shape is None else shape))
+    if t.get_device() != ctx.device:
+        raise _elsewhere(ctx, what)
+    size = t.shape
+    if len(size) != 2 or (shape is not None and size != shape):
+        raise FitreError(S.ERR_BAD_ARG, "%s must have shape %s" % (what, "(rows, cols)" if shape is None else tuple(shape)))
     if dtype is not None and t.dtype != dtype:
         raise FitreError(S.ERR_BAD_ARG, "%s must be %s" % (what, dtype))
-    rows, cols = t.shape
+    rows, cols = size
     s0, s1 = t.stride()
-    if cols > 1 and s1 != 1:
+    if s1 != 1 and cols > 1:
         raise FitreError(S.ERR_BAD_ARG, "%s must have contiguous rows" % what)
     return t.data_ptr(), s0 if rows > 1 else cols
 
@@ -554,7 +558,8 @@ def _matrix(ctx, t, what, shape=None, dtype=None):
 def _vector(ctx, t, what, n, dtype):
     if t is None:
         return None
-    _on(ctx, t, what)
+    if t.get_device() != ctx.device:
+        raise _elsewhere(ctx, what)
     if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
         raise FitreError(S.ERR_BAD_ARG, "%s must be contiguous, of %d elements of %s" % (what, n, dtype))
     return t.data_ptr()
@@ -565,25 +570,19 @@ def _scratch(ctx, t, need):
         if need:
             raise FitreError(S.ERR_WORKSPACE, "scratch of %d doubles needed, none given" % need)
         return None
-    import torch
-    _on(ctx, t, "devPtr")
-    if t.dtype != torch.float64 or not t.is_contiguous():
+    if t.get_device() != ctx.device:
+        raise _elsewhere(ctx, "devPtr")
+    if t.dtype != _TYPES["f64"] or not t.is_contiguous():
         raise FitreError(S.ERR_BAD_ARG, "device buffers must be contiguous float64 CUDA tensors")
     if t.numel() < need:
         raise FitreError(S.ERR_WORKSPACE, "scratch of %d doubles needed, %d given" % (need, t.numel()))
     return t.data_ptr()
 
 
-def _stat(t):
-    import torch
-    return torch.float64 if t.dtype == torch.float64 else torch.float32
-
-
 def _weight_dtype(t, x):
-    import torch
-    if t is None:
+    if t is None or t.dtype == x.dtype:
         return x.dtype
-    if t.dtype != x.dtype and (t.dtype != torch.float32 or x.dtype == torch.float64):
+    if t.dtype != _TYPES["f32"] or x.dtype == _TYPES["f64"]:
         raise FitreError(S.ERR_UNSUPPORTED, "weights of %s next to %s" % (t.dtype, x.dtype))
     return t.dtype
 
@@ -591,14 +590,13 @@ def _weight_dtype(t, x):
 def layerNormForward(ctx, x, gamma, beta, y, mean=None, rstd=None, eps=1e-5):
     """y = (x - mean) * rstd * gamma + beta per row; mean / rstd are kept for layerNormBackward.
     gamma / beta may be None; y may be x."""
-    code = _dtype_code(x)
+    code, stat = _kind(x)
     xp, ldx = _matrix(ctx, x, "x")
-    rows, cols = x.shape
-    yp, ldy = _matrix(ctx, y, "y", (rows, cols), x.dtype)
+    rows, cols = shape = x.shape
+    yp, ldy = _matrix(ctx, y, "y", shape, x.dtype)
     w = _weight_dtype(gamma if gamma is not None else beta, x)
-    stat = _stat(x)
     ctx.check(ctx.lib.fitre_layer_norm_forward(
-        ctx.h, code, _DTYPES[w], xp, ldx, _vector(ctx, gamma, "gamma", cols, w), _vector(ctx, beta, "beta", cols, w),
+        ctx.h, code, _KINDS[w][0], xp, ldx, _vector(ctx, gamma, "gamma", cols, w), _vector(ctx, beta, "beta", cols, w),
         yp, ldy, _vector(ctx, mean, "mean", rows, stat), _vector(ctx, rstd, "rstd", rows, stat), rows, cols, eps))
 
 
@@ -609,17 +607,16 @@ def layerNormBackwardMemRequired(rows, cols):
 
 def layerNormBackward(ctx, dy, x, gamma, mean, rstd, dx, dgamma=None, dbeta=None, devPtr=None):
     """dx, and dgamma / dbeta summed over the rows, from layerNormForward's mean and rstd."""
-    code = _dtype_code(x)
+    code, stat = _kind(x)
     xp, ldx = _matrix(ctx, x, "x")
     rows, cols = x.shape
     dyp, lddy = _matrix(ctx, dy, "dy", (rows, cols), x.dtype)
     dxp, lddx = _matrix(ctx, dx, "dx", (rows, cols), x.dtype)
     given = next((t for t in (gamma, dgamma, dbeta) if t is not None), None)
     w = _weight_dtype(given, x)
-    stat = _stat(x)
     need = layerNormBackwardMemRequired(rows, cols) if dgamma is not None or dbeta is not None else 0
     ctx.check(ctx.lib.fitre_layer_norm_backward(
-        ctx.h, code, _DTYPES[w], dyp, lddy, xp, ldx, _vector(ctx, gamma, "gamma", cols, w),
+        ctx.h, code, _KINDS[w][0], dyp, lddy, xp, ldx, _vector(ctx, gamma, "gamma", cols, w),
         _vector(ctx, mean, "mean", rows, stat), _vector(ctx, rstd, "rstd", rows, stat), dxp, lddx,
         _vector(ctx, dgamma, "dgamma", cols, w), _vector(ctx, dbeta, "dbeta", cols, w), rows, cols,
         _scratch(ctx, devPtr, need)))
@@ -628,34 +625,30 @@ def layerNormBackward(ctx, dy, x, gamma, mean, rstd, dx, dgamma=None, dbeta=None
 def tokenLogProbs(ctx, logits, tokens, logprobs=None, lse=None, entropy=None, topLogprobs=None, topTokens=None):
     """Per row of logits: log p(token), log sum exp, entropy, and (topLogprobs / topTokens of shape
     (rows, top), top <= 32) the largest alternatives, lower index first among equals."""
-    import torch
-    code = _dtype_code(logits)
+    code, stat = _kind(logits)
     xp, ld = _matrix(ctx, logits, "logits")
     rows, vocab = logits.shape
-    stat = _stat(logits)
     top = 0
     if topLogprobs is not None or topTokens is not None:
         if topLogprobs is None or topTokens is None or topTokens.dim() != 2:
             raise FitreError(S.ERR_BAD_ARG, "topLogprobs and topTokens go together, of shape (rows, top)")
         top = topTokens.shape[1]
     ctx.check(ctx.lib.fitre_token_logprobs(
-        ctx.h, code, xp, ld, _vector(ctx, tokens, "tokens", rows, torch.int64), rows, vocab,
+        ctx.h, code, xp, ld, _vector(ctx, tokens, "tokens", rows, _TYPES["i64"]), rows, vocab,
         _vector(ctx, logprobs, "logprobs", rows, stat), _vector(ctx, lse, "lse", rows, stat),
         _vector(ctx, entropy, "entropy", rows, stat), top,
         _vector(ctx, topLogprobs, "topLogprobs", rows * top, stat),
-        _vector(ctx, topTokens, "topTokens", rows * top, torch.int64)))
+        _vector(ctx, topTokens, "topTokens", rows * top, _TYPES["i64"])))
 
 
 def tokenLogProbsBackward(ctx, logits, tokens, lse, entropy, dLogprobs, dEntropy, dLogits):
     """dLogits from the gradients of tokenLogProbs' logprobs and / or entropy; dLogits may be logits."""
-    import torch
-    code = _dtype_code(logits)
+    code, stat = _kind(logits)
     xp, ld = _matrix(ctx, logits, "logits")
     rows, vocab = logits.shape
     dp, ldd = _matrix(ctx, dLogits, "dLogits", (rows, vocab), logits.dtype)
-    stat = _stat(logits)
     ctx.check(ctx.lib.fitre_token_logprobs_backward(
-        ctx.h, code, xp, ld, _vector(ctx, tokens, "tokens", rows, torch.int64), _vector(ctx, lse, "lse", rows, stat),
+        ctx.h, code, xp, ld, _vector(ctx, tokens, "tokens", rows, _TYPES["i64"]), _vector(ctx, lse, "lse", rows, stat),
         _vector(ctx, entropy, "entropy", rows, stat), _vector(ctx, dLogprobs, "dLogprobs", rows, stat),
         _vector(ctx, dEntropy, "dEntropy", rows, stat), dp, ldd, rows, vocab))
 
@@ -667,7 +660,7 @@ def gatedForwardMemRequired(tokens, width, hidden):
 
 def gatedForward(ctx, x, wGate, wUp, h, gate=None, up=None, act=S.CNN_ACT_SWISH, devPtr=None):
     """h = act(x wGate') * (x wUp'); gate / up keep the two products for gatedBackward."""
-    code = _dtype_code(x)
+    code = _kind(x)[0]
     xp, ldx = _matrix(ctx, x, "x")
     tokens, width = x.shape
     gp, ldwg = _matrix(ctx, wGate, "wGate", None, x.dtype)
@@ -690,7 +683,7 @@ def gatedBackwardMemRequired(tokens, width, hidden):
 
 def gatedBackward(ctx, dh, x, wGate, wUp, gate, up, dx, dwGate, dwUp, act=S.CNN_ACT_SWISH, devPtr=None):
     """Gradients of gatedForward from dh and the stored gate / up."""
-    code = _dtype_code(x)
+    code = _kind(x)[0]
     xp, ldx = _matrix(ctx, x, "x")
     tokens, width = x.shape
     gp, ldwg = _matrix(ctx, wGate, "wGate", None, x.dtype)
@@ -718,11 +711,10 @@ def orthogonalizeMemRequired(batch, rows, cols):
 def orthogonalizeUpdate(ctx, update, out, devPtr, steps=5, coefficients=None, scale=1.0, eps=1e-7):
     """out (bfloat16) = scale * the Newton-Schulz polynomial of update / (|update|_F + eps): one matrix
     (rows, cols) or a batch (batch, rows, cols)."""
-    import torch
-    code = _dtype_code(update)
+    code = _kind(update)[0]
     if update.dim() not in (2, 3) or tuple(out.shape) != tuple(update.shape):
         raise FitreError(S.ERR_BAD_ARG, "update and out must be matrices, or batches of matrices, of one shape")
-    if out.dtype != torch.bfloat16:
+    if out.dtype != _TYPES["bf16"]:
         raise FitreError(S.ERR_UNSUPPORTED, "out must be bfloat16")
     batch = update.shape[0] if update.dim() == 3 else 1
     if batch == 0:

@@ -64,7 +64,7 @@ struct GatedEpi {
 };
 
 // Few tokens: a warp takes one hidden unit and streams its two weight rows.
-constexpr int V_TOKENS = 4, V_THREADS = 256;
+constexpr int V_TOKENS = 4, V_THREADS = 128;   // small blocks: the last ones to finish are few
 template <class T, int NT, int VEC>
 __global__ void __launch_bounds__(V_THREADS)
 gated_few_kernel(const T *__restrict__ x, long ldx, const T *__restrict__ wg, long ldwg, const T *__restrict__ wu,
@@ -198,7 +198,7 @@ bool pairs_worth(long M, long N, int n_per_tile, int products) {
 
 template <class T, int NT, int VEC>
 void forward_few(fitre_context *ctx, const GatedArgs &a) {
-    gated_few_kernel<T, NT, VEC><<<(unsigned)((a.hidden + 7) / 8), V_THREADS, 0, ctx->stream>>>(
+    gated_few_kernel<T, NT, VEC><<<(unsigned)((a.hidden + V_THREADS / 32 - 1) / (V_THREADS / 32)), V_THREADS, 0, ctx->stream>>>(
         (const T *)a.x, a.ldx, (const T *)a.wg, a.ldwg, (const T *)a.wu, a.ldwu, (T *)a.h, a.ldh, (T *)a.g, a.ldg,
         (T *)a.u, a.ldu, (int)a.width, (int)a.hidden, a.act);
     check_launch(ctx, "gated_few_kernel");

@@ -457,29 +457,45 @@ layer_norm_backward_kernel(const T *dy, long lddy, const T *x, long ldx, const W
     }
 }
 
+// Rows on 16-byte boundaries through a ring.  A row's elements are read from shared memory twice, for the sums and for
+// dx, so that they need no registers while the block waits for the sums: three blocks fit an SM instead of two.
+constexpr int kRingThreads = 768;
 template <class T, class W, int VEC, int G>
-__global__ void __launch_bounds__(G, 512 / G > 0 ? 512 / G : 1)
+__global__ void __launch_bounds__(G, kRingThreads / G > 0 ? kRingThreads / G : 1)
 layer_norm_backward_ring_kernel(const T *dy, long lddy, const T *x, long ldx, const W *__restrict__ gamma,
                                 const acc_t<T> *__restrict__ mean, const acc_t<T> *__restrict__ rstd, T *dx, long lddx,
                                 acc_t<T> *partial, long rows, int cols, int stages, int *err) {
     using A = acc_t<T>;
-    constexpr int CH = N_ELEMS / VEC;
+    using P = SimdOf<T, VEC>;
+    constexpr int CH = N_ELEMS / VEC, PV = VEC / kPack<VEC>;
     extern __shared__ __align__(16) unsigned char ring_raw[];
     __shared__ unsigned long long bars[kRingMax];
     __shared__ A buf[4 * (G / 32)];
     const int t = threadIdx.x, bytes = cols * (int)sizeof(T);
     const long step = gridDim.x;
-    int slot = 0;
+    const A over = A(1) / (A)cols;
+    int slot = 0, before = 0;
     RowRing ring(ring_raw, bars, stages, 2 * bytes);
     ring.init();
+    // rows are fetched `stages - 1` ahead: the stage before this row's is still being read
     if (t == 0)
-        for (int i = 0; i < stages; ++i) {
+        for (int i = 0; i + 1 < stages; ++i) {
             const long r = blockIdx.x + i * step;
             if (r < rows) ring.fill2(i, x + r * ldx, dy + r * lddy);
         }
+    before = stages - 1;
     dx += t * VEC;
-    const A over = A(1) / (A)cols;
-    BackPart<T, W, VEC, G, CH> part(cols, t, gamma ? gamma + t * VEC : gamma);
+    const int left = cols - t * VEC;   // chunk c exists while c * G * VEC < left
+    P dg[CH][PV], db[CH][PV];
+    Vec<W, VEC> gm[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+#pragma unroll
+        for (int i = 0; i < PV; ++i) dg[c][i] = db[c][i] = P::splat(A(0));
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) gm[c].v[e] = from_acc<W>(A(1));
+        if (gamma && c * G * VEC < left) gm[c] = load_vec<W, VEC>(gamma + (c * G + t) * VEC);
+    }
     for (long row = blockIdx.x; row < rows; row += step) {
         const A m = mean[row], r = rstd[row];
         if (!ring.wait()) {
@@ -487,18 +503,60 @@ layer_norm_backward_ring_kernel(const T *dy, long lddy, const T *x, long ldx, co
             return;
         }
         const T *xs = (const T *)ring.data() + t * VEC, *ds = (const T *)(ring.data() + bytes) + t * VEC;
-        A s1, s2;
-        part.take(m, r, [&](int c) { return load_vec<T, VEC>(xs + c * G * VEC); },
-                  [&](int c) { return load_vec<T, VEC>(ds + c * G * VEC); }, s1, s2);
+        const P scale = P::splat(r), shift = P::splat(-m * r);
+        P a = P::splat(A(0)), b = a;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+            if (c * G * VEC < left) {
+                P xh[PV], d[PV], w[PV];
+                widen(load_vec<T, VEC>(xs + c * G * VEC), xh);
+                widen(load_vec<T, VEC>(ds + c * G * VEC), d);
+                widen(gm[c], w);
+#pragma unroll
+                for (int i = 0; i < PV; ++i) {
+                    xh[i] = fma(xh[i], scale, shift);
+                    dg[c][i] = fma(d[i], xh[i], dg[c][i]);
+                    db[c][i] = add(db[c][i], d[i]);
+                    const P g = mul(d[i], w[i]);
+                    a = add(a, g);
+                    b = fma(g, xh[i], b);
+                }
+            }
+        A s1 = a.sum(), s2 = b.sum();
         group_sum2<G>(s1, s2, buf, slot);
-        if (t == 0 && row + stages * step < rows)
-            ring.fill2(ring.at, x + (row + stages * step) * ldx, dy + (row + stages * step) * lddy);
+        // past the sums' barrier no thread reads the stage of the row before this one
+        if (t == 0 && row + (stages - 1) * step < rows)
+            ring.fill2(before, x + (row + (stages - 1) * step) * ldx, dy + (row + (stages - 1) * step) * lddy);
+        before = ring.at;
         ring.advance();
-        part.store(r, s1 * over, s2 * over, dx + row * lddx);
+        // dx = r (g - s1 - xh s2), s1 and s2 as means
+        s1 *= over;
+        s2 *= over;
+        const P back1 = P::splat(-s1 * r), back2 = P::splat(-s2 * r);
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+            if (c * G * VEC < left) {
+                P xh[PV], d[PV], w[PV];
+                widen(load_vec<T, VEC>(xs + c * G * VEC), xh);
+                widen(load_vec<T, VEC>(ds + c * G * VEC), d);
+                widen(gm[c], w);
+#pragma unroll
+                for (int i = 0; i < PV; ++i)
+                    d[i] = fma(fma(xh[i], scale, shift), back2, fma(mul(d[i], w[i]), scale, back1));
+                store_vec<T, VEC>(dx + row * lddx + c * G * VEC, narrowed<T, VEC>(d));
+            }
     }
     if (!partial) return;
-    A *pg = partial + (long)blockIdx.x * 2 * cols + t * VEC;
-    part.flush(pg, pg + cols);
+    A *pg = partial + (long)blockIdx.x * 2 * cols + t * VEC, *pb = pg + cols;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+        if (c * G * VEC < left) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                pg[c * G * VEC + e] = dg[c][e / kPack<VEC>].get(e % kPack<VEC>);
+                pb[c * G * VEC + e] = db[c][e / kPack<VEC>].get(e % kPack<VEC>);
+            }
+        }
 }
 
 // Column sums for rows too long for registers: a block takes 256 columns and every gridDim.y-th row.
@@ -664,9 +722,9 @@ void backward_as(fitre_context *ctx, const NormArgs &a) {
     A *partial = a.dgamma || a.dbeta ? (A *)a.scratch : nullptr;
     int blocks = blocks_for(a.rows, g ? g : 1024, kBackThreads);
     const long bytes = 2l * a.cols * sizeof(T);
-    const int stages = VEC > 1 && g > 32 ? ring_stages(g, kBackThreads, bytes) : 0;
+    const int stages = VEC > 1 && g > 32 ? ring_stages(g, kRingThreads, bytes) : 0;
     if constexpr (VEC > 1) if (stages) {
-        blocks = blocks_for(a.rows, g, kBackThreads);
+        blocks = blocks_for(a.rows, g, kRingThreads);
 #define NORM_LAUNCH(G)                                                                                       \
     allow_shared(layer_norm_backward_ring_kernel<T, W, VEC, G>, stages * bytes);                             \
     layer_norm_backward_ring_kernel<T, W, VEC, G><<<blocks, G, stages * bytes, ctx->stream>>>(               \
@@ -753,7 +811,7 @@ void norm_dispatch(fitre_context *ctx, const NormArgs &a, bool back) {
 
 long layer_norm_backward_scratch(long rows, long cols) {
     const int g = cols <= 1024 * N_ELEMS ? group_for((int)cols) : 0;
-    const long parts = g ? blocks_for(rows, g, kBackThreads) : (rows < kLongSplit ? rows : kLongSplit);
+    const long parts = g ? blocks_for(rows, g, kRingThreads) : (rows < kLongSplit ? rows : kLongSplit);
     return parts * 2 * cols * (long)sizeof(double);
 }
 void layer_norm_forward(fitre_context *ctx, const NormArgs &a) { norm_dispatch(ctx, a, false); }
