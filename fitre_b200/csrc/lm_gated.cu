@@ -12,6 +12,7 @@
 // concatenated inner dimension, and dWg / dWu one launch over both.
 // All sums are fp32; each output is rounded once.
 #include "lm_gemm.cuh"
+#include "lm_simd.cuh"
 
 namespace fitre {
 namespace {
@@ -69,40 +70,54 @@ template <class T, int NT, int VEC>
 __global__ void __launch_bounds__(V_THREADS)
 gated_few_kernel(const T *__restrict__ x, long ldx, const T *__restrict__ wg, long ldwg, const T *__restrict__ wu,
                  long ldwu, T *h, long ldh, T *g_out, long ldg, T *u_out, long ldu, int D, int F, int act) {
+    using P = SimdOf<T, VEC>;
+    constexpr int PV = VEC / kPack<VEC>, DEEP = 4;   // loads of each weight row a lane has in flight
     const int lane = threadIdx.x & 31, f = (blockIdx.x * V_THREADS + threadIdx.x) / 32;
-    if (f < F) {
-        float g[NT], u[NT];
+    if (f >= F) return;
+    P gs[NT], us[NT];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) g[t] = u[t] = 0.0f;
-        const T *pg = wg + (long)f * ldwg, *pu = wu + (long)f * ldwu;
-#pragma unroll 4
-        for (int d = lane * VEC; d < D; d += 32 * VEC) {
-            const Vec<T, VEC> a = load_vec<T, VEC>(pg + d), b = load_vec<T, VEC>(pu + d);
+    for (int t = 0; t < NT; ++t) gs[t] = us[t] = P::splat(0.0f);
+    const T *pg = wg + (long)f * ldwg + lane * VEC, *pu = wu + (long)f * ldwu + lane * VEC;
+    x += lane * VEC;
+    const int left = D - lane * VEC;   // this lane's elements start at multiples of 32 VEC below it
+    for (int d0 = 0; d0 < left; d0 += DEEP * 32 * VEC) {
+        Vec<T, VEC> a[DEEP], b[DEEP];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const Vec<T, VEC> xv = load_vec<T, VEC>(x + t * ldx + d);
+        for (int i = 0; i < DEEP; ++i)
+            if (d0 + i * 32 * VEC < left) {
+                a[i] = load_vec<T, VEC>(pg + d0 + i * 32 * VEC);
+                b[i] = load_vec<T, VEC>(pu + d0 + i * 32 * VEC);
+            }
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float xe = to_acc<float>(xv.v[e]);
-                    g[t] += to_acc<float>(a.v[e]) * xe;
-                    u[t] += to_acc<float>(b.v[e]) * xe;
+        for (int i = 0; i < DEEP; ++i)
+            if (d0 + i * 32 * VEC < left) {
+                P av[PV], bv[PV], xv[PV];
+                widen(a[i], av);
+                widen(b[i], bv);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    widen(load_vec<T, VEC>(x + t * ldx + d0 + i * 32 * VEC), xv);
+#pragma unroll
+                    for (int j = 0; j < PV; ++j) {
+                        gs[t] = fma(av[j], xv[j], gs[t]);
+                        us[t] = fma(bv[j], xv[j], us[t]);
+                    }
                 }
             }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        float g = gs[t].sum(), u = us[t].sum();
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            g += __shfl_xor_sync(0xffffffffu, g, o);
+            u += __shfl_xor_sync(0xffffffffu, u, o);
         }
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                g[t] += __shfl_xor_sync(0xffffffffu, g[t], o);
-                u[t] += __shfl_xor_sync(0xffffffffu, u[t], o);
-            }
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-            if (lane == t) {
-                if (g_out) g_out[t * ldg + f] = from_acc<T>(g[t]);
-                if (u_out) u_out[t * ldu + f] = from_acc<T>(u[t]);
-                h[t * ldh + f] = from_acc<T>(act_value(act, g[t]) * u[t]);
-            }
+        if (lane == t) {
+            if (g_out) g_out[t * ldg + f] = from_acc<T>(g);
+            if (u_out) u_out[t * ldu + f] = from_acc<T>(u);
+            h[t * ldh + f] = from_acc<T>(act_value(act, g) * u);
+        }
     }
 }
 

@@ -51,6 +51,28 @@ __device__ __forceinline__ void group_sum2(A &a, A &b, A *buf, int &slot) {
     }
 }
 
+// The same for N values at once.
+template <int G, int N, class A>
+__device__ __forceinline__ void group_sums(A (&v)[N], A *buf, int &slot) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    constexpr int W = G / 32;
+    A *s = buf + slot * N * W;
+    slot ^= 1;
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[(threadIdx.x >> 5) * N + i] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += s[w * N + i];
+}
 template <int G, class A>
 __device__ __forceinline__ A group_sum(A a, A *buf, int &slot) {
 #pragma unroll
@@ -457,10 +479,11 @@ layer_norm_backward_kernel(const T *dy, long lddy, const T *x, long ldx, const W
     }
 }
 
-// Rows on 16-byte boundaries through a ring.  A row's elements are read from shared memory twice, for the sums and for
-// dx, so that they need no registers while the block waits for the sums: three blocks fit an SM instead of two.
-constexpr int kRingThreads = 768;
-template <class T, class W, int VEC, int G>
+// Rows on 16-byte boundaries through a ring, R (1 or 2) rows at a time: two rows share one barrier and hide one
+// another's latencies.  Elements are read from shared memory twice, for the sums and for dx, so that they need no
+// registers while the block waits for the sums.
+constexpr int kRingThreads = 512;   // resident threads per SM
+template <class T, class W, int VEC, int G, int R>
 __global__ void __launch_bounds__(G, kRingThreads / G > 0 ? kRingThreads / G : 1)
 layer_norm_backward_ring_kernel(const T *dy, long lddy, const T *x, long ldx, const W *__restrict__ gamma,
                                 const acc_t<T> *__restrict__ mean, const acc_t<T> *__restrict__ rstd, T *dx, long lddx,
@@ -470,20 +493,22 @@ layer_norm_backward_ring_kernel(const T *dy, long lddy, const T *x, long ldx, co
     constexpr int CH = N_ELEMS / VEC, PV = VEC / kPack<VEC>;
     extern __shared__ __align__(16) unsigned char ring_raw[];
     __shared__ unsigned long long bars[kRingMax];
-    __shared__ A buf[4 * (G / 32)];
+    __shared__ A buf[4 * R * (G / 32)];
     const int t = threadIdx.x, bytes = cols * (int)sizeof(T);
-    const long step = gridDim.x;
+    const long apart = gridDim.x, step = apart * R;   // between a block's rows, between its groups of rows
     const A over = A(1) / (A)cols;
-    int slot = 0, before = 0;
-    RowRing ring(ring_raw, bars, stages, 2 * bytes);
+    int slot = 0, before = stages - 1;
+    RowRing ring(ring_raw, bars, stages, 2 * R * bytes);
     ring.init();
-    // rows are fetched `stages - 1` ahead: the stage before this row's is still being read
+    auto count = [&](long row) {   // rows of the group that starts at `row`
+        return row >= rows ? 0 : R == 2 && row + apart < rows ? 2 : 1;
+    };
+    // groups are fetched `stages - 1` ahead: the stage of the group before this one is still being read
     if (t == 0)
         for (int i = 0; i + 1 < stages; ++i) {
             const long r = blockIdx.x + i * step;
-            if (r < rows) ring.fill2(i, x + r * ldx, dy + r * lddy);
+            if (count(r)) ring.fill_pairs(i, x, ldx, dy, lddy, r, apart, count(r), bytes);
         }
-    before = stages - 1;
     dx += t * VEC;
     const int left = cols - t * VEC;   // chunk c exists while c * G * VEC < left
     P dg[CH][PV], db[CH][PV];
@@ -496,54 +521,85 @@ layer_norm_backward_ring_kernel(const T *dy, long lddy, const T *x, long ldx, co
         for (int e = 0; e < VEC; ++e) gm[c].v[e] = from_acc<W>(A(1));
         if (gamma && c * G * VEC < left) gm[c] = load_vec<W, VEC>(gamma + (c * G + t) * VEC);
     }
+    A next_m[R], next_r[R];
+    auto statistics = [&](long row) {
+#pragma unroll
+        for (int k = 0; k < R; ++k)
+            if (row + k * apart < rows) {
+                next_m[k] = mean[row + k * apart];
+                next_r[k] = rstd[row + k * apart];
+            }
+    };
+    statistics(blockIdx.x);
     for (long row = blockIdx.x; row < rows; row += step) {
-        const A m = mean[row], r = rstd[row];
+        const int n = count(row);
+        A m[R], r[R], s[2 * R];
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            m[k] = next_m[k];
+            r[k] = next_r[k];
+            s[2 * k] = s[2 * k + 1] = 0;
+        }
+        statistics(row + step);   // travel meanwhile
         if (!ring.wait()) {
             if (t == 0) atomicExch(err, 1);
             return;
         }
-        const T *xs = (const T *)ring.data() + t * VEC, *ds = (const T *)(ring.data() + bytes) + t * VEC;
-        const P scale = P::splat(r), shift = P::splat(-m * r);
-        P a = P::splat(A(0)), b = a;
+        const T *in = (const T *)ring.data() + t * VEC;
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
-            if (c * G * VEC < left) {
-                P xh[PV], d[PV], w[PV];
-                widen(load_vec<T, VEC>(xs + c * G * VEC), xh);
-                widen(load_vec<T, VEC>(ds + c * G * VEC), d);
-                widen(gm[c], w);
+        for (int k = 0; k < R; ++k)
+            if (k < n) {
+                const T *xs = in + 2 * k * cols, *ds = xs + cols;
+                const P scale = P::splat(r[k]), shift = P::splat(-m[k] * r[k]);
+                P a = P::splat(A(0)), b = a;
 #pragma unroll
-                for (int i = 0; i < PV; ++i) {
-                    xh[i] = fma(xh[i], scale, shift);
-                    dg[c][i] = fma(d[i], xh[i], dg[c][i]);
-                    db[c][i] = add(db[c][i], d[i]);
-                    const P g = mul(d[i], w[i]);
-                    a = add(a, g);
-                    b = fma(g, xh[i], b);
-                }
+                for (int c = 0; c < CH; ++c)
+                    if (c * G * VEC < left) {
+                        P xh[PV], d[PV], w[PV];
+                        widen(load_vec<T, VEC>(xs + c * G * VEC), xh);
+                        widen(load_vec<T, VEC>(ds + c * G * VEC), d);
+                        widen(gm[c], w);
+#pragma unroll
+                        for (int i = 0; i < PV; ++i) {
+                            xh[i] = fma(xh[i], scale, shift);
+                            dg[c][i] = fma(d[i], xh[i], dg[c][i]);
+                            db[c][i] = add(db[c][i], d[i]);
+                            const P g = mul(d[i], w[i]);
+                            a = add(a, g);
+                            b = fma(g, xh[i], b);
+                        }
+                    }
+                s[2 * k] = a.sum();
+                s[2 * k + 1] = b.sum();
             }
-        A s1 = a.sum(), s2 = b.sum();
-        group_sum2<G>(s1, s2, buf, slot);
-        // past the sums' barrier no thread reads the stage of the row before this one
-        if (t == 0 && row + (stages - 1) * step < rows)
-            ring.fill2(before, x + (row + (stages - 1) * step) * ldx, dy + (row + (stages - 1) * step) * lddy);
+        group_sums<G>(s, buf, slot);
+        // past the sums' barrier no thread reads the stage of the group before this one
+        if (t == 0) {
+            const long ahead = row + (stages - 1) * step;
+            if (count(ahead)) ring.fill_pairs(before, x, ldx, dy, lddy, ahead, apart, count(ahead), bytes);
+        }
         before = ring.at;
         ring.advance();
-        // dx = r (g - s1 - xh s2), s1 and s2 as means
-        s1 *= over;
-        s2 *= over;
-        const P back1 = P::splat(-s1 * r), back2 = P::splat(-s2 * r);
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
-            if (c * G * VEC < left) {
-                P xh[PV], d[PV], w[PV];
-                widen(load_vec<T, VEC>(xs + c * G * VEC), xh);
-                widen(load_vec<T, VEC>(ds + c * G * VEC), d);
-                widen(gm[c], w);
+        for (int k = 0; k < R; ++k)
+            if (k < n) {
+                // dx = r (g - s1 - xh s2), s1 and s2 as means
+                const T *xs = in + 2 * k * cols, *ds = xs + cols;
+                T *to = dx + (row + k * apart) * lddx;
+                const P scale = P::splat(r[k]), shift = P::splat(-m[k] * r[k]);
+                const P back1 = P::splat(-s[2 * k] * over * r[k]), back2 = P::splat(-s[2 * k + 1] * over * r[k]);
 #pragma unroll
-                for (int i = 0; i < PV; ++i)
-                    d[i] = fma(fma(xh[i], scale, shift), back2, fma(mul(d[i], w[i]), scale, back1));
-                store_vec<T, VEC>(dx + row * lddx + c * G * VEC, narrowed<T, VEC>(d));
+                for (int c = 0; c < CH; ++c)
+                    if (c * G * VEC < left) {
+                        P xh[PV], d[PV], w[PV];
+                        widen(load_vec<T, VEC>(xs + c * G * VEC), xh);
+                        widen(load_vec<T, VEC>(ds + c * G * VEC), d);
+                        widen(gm[c], w);
+#pragma unroll
+                        for (int i = 0; i < PV; ++i)
+                            d[i] = fma(fma(xh[i], scale, shift), back2, fma(mul(d[i], w[i]), scale, back1));
+                        store_vec<T, VEC>(to + c * G * VEC, narrowed<T, VEC>(d));
+                    }
             }
     }
     if (!partial) return;
@@ -722,18 +778,27 @@ void backward_as(fitre_context *ctx, const NormArgs &a) {
     A *partial = a.dgamma || a.dbeta ? (A *)a.scratch : nullptr;
     int blocks = blocks_for(a.rows, g ? g : 1024, kBackThreads);
     const long bytes = 2l * a.cols * sizeof(T);
-    const int stages = VEC > 1 && g > 32 ? ring_stages(g, kRingThreads, bytes) : 0;
+    // two rows at a time where three stages of them fit (not in rows above 8192 elements), else one
+    const int two = VEC > 1 && g > 32 && g < 1024 ? ring_stages(g, kRingThreads, 2 * bytes) : 0;
+    const int stages = two >= 3 ? two : VEC > 1 && g > 32 ? ring_stages(g, kRingThreads, bytes) : 0;
     if constexpr (VEC > 1) if (stages) {
         blocks = blocks_for(a.rows, g, kRingThreads);
-#define NORM_LAUNCH(G)                                                                                       \
-    allow_shared(layer_norm_backward_ring_kernel<T, W, VEC, G>, stages * bytes);                             \
-    layer_norm_backward_ring_kernel<T, W, VEC, G><<<blocks, G, stages * bytes, ctx->stream>>>(               \
-        dy, a.lddy, x, a.ldx, gm, mean, rstd, dx, a.lddx, partial, a.rows, a.cols, stages, (int *)(ctx->dscal + 4000))
-        switch (g) {
-            case 128: NORM_LAUNCH(128); break;
-            case 256: NORM_LAUNCH(256); break;
-            case 512: NORM_LAUNCH(512); break;
-            default: NORM_LAUNCH(1024); break;
+#define NORM_LAUNCH(G, R)                                                                                    \
+    do {                                                                                                     \
+        allow_shared(layer_norm_backward_ring_kernel<T, W, VEC, G, R>, stages * R * bytes);                  \
+        layer_norm_backward_ring_kernel<T, W, VEC, G, R><<<blocks, G, stages * R * bytes, ctx->stream>>>(    \
+            dy, a.lddy, x, a.ldx, gm, mean, rstd, dx, a.lddx, partial, a.rows, a.cols, stages,               \
+            (int *)(ctx->dscal + 4000));                                                                     \
+    } while (0)
+        if (two >= 3) {
+            if (g == 128) NORM_LAUNCH(128, 2);
+            else if (g == 256) NORM_LAUNCH(256, 2);
+            else NORM_LAUNCH(512, 2);
+        } else {
+            if (g == 128) NORM_LAUNCH(128, 1);
+            else if (g == 256) NORM_LAUNCH(256, 1);
+            else if (g == 512) NORM_LAUNCH(512, 1);
+            else NORM_LAUNCH(1024, 1);
         }
 #undef NORM_LAUNCH
         check_launch(ctx, "layer_norm_backward_ring_kernel");

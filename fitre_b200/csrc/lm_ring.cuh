@@ -37,12 +37,16 @@ struct RowRing {
         mbar_expect_tx(bar, bytes);
         bulk_load(smem_u32(base + (size_t)i * bytes), src, bytes, bar);
     }
-    // two rows of equal length, one after the other
-    __device__ __forceinline__ void fill2(int i, const void *a, const void *b) {
+    // `n` rows of a pair of matrices, `each` bytes a row and `step` rows apart: a's and b's rows in turn
+    template <class T>
+    __device__ __forceinline__ void fill_pairs(int i, const T *a, long lda, const T *b, long ldb, long row, long step, int n,
+                                               int each) {
         const uint32_t bar = smem_u32(bars + i), dst = smem_u32(base + (size_t)i * bytes);
-        mbar_expect_tx(bar, bytes);
-        bulk_load(dst, a, bytes / 2, bar);
-        bulk_load(dst + bytes / 2, b, bytes / 2, bar);
+        mbar_expect_tx(bar, 2 * n * each);
+        for (int k = 0; k < n; ++k) {
+            bulk_load(dst + 2 * k * each, a + (row + k * step) * lda, each, bar);
+            bulk_load(dst + (2 * k + 1) * each, b + (row + k * step) * ldb, each, bar);
+        }
     }
     // false: the bounded wait ran out
     __device__ __forceinline__ bool wait() const { return mbar_wait(smem_u32(bars + at), phase); }
