@@ -53,8 +53,8 @@ struct GatedEpi {
 #pragma unroll 1
         for (int c = 0; c < width && first + c < p.h.cols; c += 64) {
             float g[64], u[64];
-            tmem_load64(tmem + c, g);
-            tmem_load64(tmem + width + c, u);
+            st.sums(tmem, c, g);
+            st.sums(tmem, width + c, u);
             if (p.g.out) st.put(p.g, row0, first + c, 0, g);
             if (p.u.out) st.put(p.u, row0, first + c, 0, u);
 #pragma unroll
@@ -130,7 +130,9 @@ gated_slopes_kernel(const T *dh, long lddh, const T *g, long ldg, const T *u, lo
     const long row = blockIdx.y;
     const int at = (blockIdx.x * 256 + threadIdx.x) * VEC;
     if (at >= F) {
-        if (VEC == 1 && at < ld) out[row * ld + at] = out[half + row * ld + at] = from_acc<T>(0.0f);
+        if (VEC < 8)
+            for (int e = 0; e < VEC; ++e)
+                if (at + e < ld) out[row * ld + at + e] = out[half + row * ld + at + e] = from_acc<T>(0.0f);
         return;
     }
     const Vec<T, VEC> a = load_vec<T, VEC>(dh + row * lddh + at), b = load_vec<T, VEC>(g + row * ldg + at),
@@ -285,7 +287,11 @@ void backward_as(fitre_context *ctx, const GatedArgs &a) {
     T *slopes = (T *)a.scratch;
     char *room = (char *)a.scratch + up128(2 * 2 * half);
     const bool wide = a.hidden % 8 == 0 && tma_readable(a.dh, a.lddh) && tma_readable(a.g, a.ldg) && tma_readable(a.u, a.ldu);
-    wide ? slopes_as<T, 8>(ctx, a, slopes, ld, half) : slopes_as<T, 1>(ctx, a, slopes, ld, half);
+    const bool even = a.hidden % 2 == 0 && ((uintptr_t)a.dh | (uintptr_t)a.g | (uintptr_t)a.u) % 4 == 0 &&
+                      (a.lddh | a.ldg | a.ldu) % 2 == 0;
+    if (wide) slopes_as<T, 8>(ctx, a, slopes, ld, half);
+    else if (even) slopes_as<T, 2>(ctx, a, slopes, ld, half);
+    else slopes_as<T, 1>(ctx, a, slopes, ld, half);
     const Operands<T> o = readable<T>(ctx, a, room);
     if (pairs_worth(a.tokens, a.width, 256, 1)) input_gradient<T, 2, 256>(ctx, a, o, slopes, ld, half);
     else input_gradient<T, 1, 128>(ctx, a, o, slopes, ld, half);

@@ -15,7 +15,9 @@
 //              columns in shared memory and sends them off as one TMA store: full cache lines, edges clipped.
 // CG = 2 pairs two SMs on a 256 x BN tile: each CTA loads its 128 rows of A and half of B's rows, so a byte
 // of B feeds twice the arithmetic; the even CTA's issuer drives both.  CG = 1 (128 x BN) is for products
-// with too few tiles to occupy the pairs.  Every wait is bounded; when one runs out, the CTA sets the
+// with too few tiles to occupy the pairs; where even those leave SMs idle, a cluster of 2 or 4 CTAs divides a tile's k
+// among itself and each CTA adds up and stores a part of the tile's rows, from the others' partial sums in its
+// shared memory (1003 x 1000 x 5460: 39 -> 18 us against halving the tiles).  Every wait is bounded; when one runs out, the CTA sets the
 // context's error word, lets its copies in flight land, frees its TMEM and returns.
 #pragma once
 
@@ -36,6 +38,7 @@ struct TileGrid {
     int per;              // tiles per product
     int triangle;         // 1: only tiles with column <= row (the product is symmetric)
     int kblocks, nseg;    // stages per segment, segments (map index = segment)
+    int split;            // CTAs (a cluster) that share a tile's k; then there are no more tiles than clusters
     int za, zb;           // 1: the batch index is the operand map's third coordinate
     uint32_t idesc, idesc_half;
     int *err;
@@ -218,6 +221,19 @@ struct Stager {
     int lane, turn;
     uint32_t phase;
     bool loading;
+    uint32_t partial;   // other CTAs' sums for this warp's rows, `parts` blocks of [128 columns][32 rows]
+    int parts;
+    // 64 accumulator columns of this thread's row, the first of them column `c` of the tile at `tmem`
+    __device__ __forceinline__ void sums(uint32_t tmem, int c, float (&v)[64]) const {
+        tmem_load64(tmem + c, v);
+        for (int s = 0; s < parts; ++s)
+#pragma unroll
+            for (int e = 0; e < 64; ++e) {
+                float o;
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(o) : "r"(partial + s * 16384 + (c + e) * 128 + lane * 4));
+                v[e] += o;
+            }
+    }
     // The next of the two buffers, once its last store has read it.
     __device__ __forceinline__ uint32_t next() {
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
@@ -381,8 +397,9 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t rank = CG == 2 ? cluster_rank() : 0;
     const TileGrid &g = p.g;
-    const int first = blockIdx.x / CG, step = gridDim.x / CG;
-    const int iters = g.nseg * g.kblocks;
+    const int split = CG == 1 ? g.split : 1, part = split > 1 ? (int)cluster_rank() : 0;
+    const int first = blockIdx.x / (CG * split), step = gridDim.x / (CG * split);
+    const int all = g.nseg * g.kblocks, it0 = all * part / split, iters = all * (part + 1) / split - it0;
 
     if (tid == 0) {
         *gave_up = 0;
@@ -426,7 +443,7 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
         bool ok = true;
         const uint32_t full0 = smem_u32(bars), free0 = smem_u32(bars + 8), data0 = smem_u32(sm);
         const uint32_t land0 = CG == 2 ? map_to_rank(full0, 0) : full0;   // both CTAs' loads count on the even one's
-        const int kblocks = g.kblocks, nseg = g.nseg;
+        const int kblocks = g.kblocks;
         for (int t = first; ok && t < g.total; t += step) {
             const TileAt at = tile_at(g, t);
             const int za = g.za ? at.batch : 0, zb = g.zb ? at.batch : 0;
@@ -435,9 +452,10 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
             const int shift = at.half > 0 ? 1 : 0, rows = at.half < 0 ? L::BROWS : L::BROWS / 2;
             const int brow = Epi::kTwoMaps ? at.n * (BN / 2) + shift * (BN / 4)
                                            : at.n * BN + shift * (BN / 2) + (int)rank * rows;
-            for (int seg = 0; ok && seg < nseg; ++seg) {
+            int seg = it0 / kblocks, kb = it0 - seg * kblocks, left = iters;
+            for (; ok && left > 0; ++seg, kb = 0) {
                 const Operand &oa = p.a[seg], &ob = p.b[Epi::kTwoMaps ? (int)rank : seg];
-                for (int kb = 0, k = 0; kb < kblocks; ++kb, k += G_KB) {
+                for (int k = kb * G_KB; kb < kblocks && left > 0; ++kb, --left, k += G_KB) {
                     if (!mbar_wait_bounded(free0 + s * 8, phase)) {
                         ok = false;
                         break;
@@ -506,11 +524,12 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
             if (ok) mma_commit<CG>(smem_u32(bars + 16 + buf));
         }
         if (!ok) *gave_up = 1;
-    } else if (warp >= 2) {
+    }
+    const int quarter = warp & 3;   // the TMEM lanes an epilogue warp may read
+    Stager stager{smem_u32(sm + ST * L::STAGE) + quarter * 8192, smem_u32(bars + 22 + quarter), gave_up, lane, 0, 0, false, 0, 0};
+    if (warp >= 2 && split == 1) {
         // ---------------- epilogue ----------------
-        const int quarter = warp & 3;   // the TMEM lanes this warp may read
         const uint32_t freed = CG == 2 ? map_to_rank(smem_u32(bars + 18), 0) : smem_u32(bars + 18);
-        Stager stager{smem_u32(sm + ST * L::STAGE) + (warp - 2) * 8192, smem_u32(bars + 22 + (warp - 2)), gave_up, lane, 0, 0, false};
         int n = 0;
         for (int t = first; t < g.total; t += step, ++n) {
             const int buf = n & 1;
@@ -530,6 +549,42 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
                 else mbar_arrive(freed + buf * 8);
             }
         }
+    } else if (split > 1) {
+        // ---------------- one tile, its k divided among the cluster ----------------
+        bool done = true;
+        if (warp >= 2) done = mbar_wait_bounded(smem_u32(bars + 16), 0);
+        if (!done) *gave_up = 1;
+        __syncwarp();
+        cluster_barrier();   // every CTA's stages are free
+        const int owner = quarter * split / 4, own = 4 / split;   // who adds up these 32 rows; row quarters per CTA
+        const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t room = smem_u32(sm) + (quarter % own) * (split - 1) * 16384;
+        if (warp >= 2) {
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (owner != part) {
+                const uint32_t to = map_to_rank(room + (part < owner ? part : part - 1) * 16384, owner) + lane * 4;
+#pragma unroll 1
+                for (int c = 0; c < BN; c += 64) {
+                    float v[64];
+                    tmem_load64(mine + c, v);
+#pragma unroll
+                    for (int e = 0; e < 64; ++e)
+                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + (c + e) * 128), "f"(v[e]) : "memory");
+                }
+            }
+        }
+        __syncwarp();
+        cluster_barrier();   // the partial sums have arrived
+        if (warp >= 2 && owner == part) {
+            const TileAt at = tile_at(g, first);
+            const int row0 = at.m * 128 + quarter * 32;
+            stager.partial = room;
+            stager.parts = split - 1;
+            Epi::template begin<BN>(p.epi, at, row0, stager);
+            Epi::template store<BN>(p.epi, at, row0, mine, stager);
+        }
+    }
+    if (warp >= 2) {
         stager.drain();
         stager.settle();
     }
@@ -562,7 +617,7 @@ struct StoreEpi {
 #pragma unroll 1
         for (int c = 0; c < width && first + c < o.cols; c += 64) {
             float v[64];
-            tmem_load64(tmem + c, v);
+            st.sums(tmem, c, v);
             st.put(o, row0, first + c, 0, v);
         }
     }
@@ -637,6 +692,13 @@ void gemm_launch(fitre_context *ctx, GemmArgs<typename Epi::Params> &args, int M
     const int room = kLmSms / CG, tiles = (int)per * batch, left = tiles % room;
     // (64 columns are the least an epilogue stores at a time; two maps on one SM load no half tiles)
     g.whole = left > 0 && left <= room / 2 && !(Epi::kTwoMaps && CG == 1) ? tiles - left : tiles;
+    // dividing k is worth its exchange of partial sums from a few stages per CTA on
+    const int stages = (int)((K + G_KB - 1) / G_KB) * nseg;
+    g.split = 1;
+    if (CG == 1 && tiles <= kLmSms / 2 && stages >= 8) {
+        g.split = tiles <= kLmSms / 4 && stages >= 16 ? 4 : 2;
+        g.whole = tiles;
+    }
     g.total = g.whole + 2 * (tiles - g.whole);
     g.triangle = triangle;
     g.kblocks = (int)((K + G_KB - 1) / G_KB);
@@ -650,13 +712,13 @@ void gemm_launch(fitre_context *ctx, GemmArgs<typename Epi::Params> &args, int M
         ready = ctx->device;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((g.total < room ? g.total : room) * CG));
+    cfg.gridDim = dim3((unsigned)((g.total < room ? g.total : room) * CG * g.split));
     cfg.blockDim = dim3(G_THREADS);
     cfg.dynamicSmemBytes = L::SMEM;
     cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CG;
+    attr[0].val.clusterDim.x = (unsigned)(CG * g.split);
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;

@@ -116,7 +116,7 @@ struct SymmetricEpi {
             const int col = first + c;
             if (p.with_in && c > 0) st.load(&p.in, nullptr, col, row0, at.batch);
             float acc[64];
-            tmem_load64(tmem + c, acc);
+            st.sums(tmem, c, acc);
             if (p.with_in) st.wait();
             const int on = p.diag && row < n ? row - col : -1;   // this row's diagonal element in the block, if 0..63
             uint32_t w[32];
@@ -187,7 +187,7 @@ struct IterateEpi {
         for (int c = 0; c < width && first + c < p.out.cols; c += 64) {
             const int col = first + c, left = p.cols - col;
             float acc[64];
-            tmem_load64(tmem + c, acc);
+            st.sums(tmem, c, acc);
             st.wait();
             uint32_t w[32], r[32];
 #pragma unroll
