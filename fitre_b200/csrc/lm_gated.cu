@@ -17,9 +17,17 @@
 namespace fitre {
 namespace {
 
+// 1 / (1 + exp(-g)) to 2^-21 by the fast exponential and reciprocal: outputs have 11 bits at most, and with exact
+// division the epilogue would take longer than a short product.
+__device__ __forceinline__ float sigmoid(float g) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return r;
+}
 __device__ __forceinline__ float act_value(int act, float g) {
     switch (act) {
-        case FITRE_CNN_ACT_SWISH: return g / (1.0f + __expf(-g));
+        case FITRE_CNN_ACT_SWISH: return g * sigmoid(g);
         case FITRE_CNN_ACT_RELU: return fmaxf(g, 0.0f);
         case FITRE_CNN_ACT_SOFTPLUS: return fmaxf(g, 0.0f) + log1pf(__expf(-fabsf(g)));
         default: return g;
@@ -28,11 +36,11 @@ __device__ __forceinline__ float act_value(int act, float g) {
 __device__ __forceinline__ float act_slope(int act, float g) {
     switch (act) {
         case FITRE_CNN_ACT_SWISH: {
-            const float s = 1.0f / (1.0f + __expf(-g));
+            const float s = sigmoid(g);
             return s * (1.0f + g * (1.0f - s));
         }
         case FITRE_CNN_ACT_RELU: return g > 0.0f ? 1.0f : 0.0f;
-        case FITRE_CNN_ACT_SOFTPLUS: return 1.0f / (1.0f + __expf(-g));
+        case FITRE_CNN_ACT_SOFTPLUS: return sigmoid(g);
         default: return 1.0f;
     }
 }
@@ -57,8 +65,13 @@ struct GatedEpi {
             st.sums(tmem, width + c, u);
             if (p.g.out) st.put(p.g, row0, first + c, 0, g);
             if (p.u.out) st.put(p.u, row0, first + c, 0, u);
+            if (p.act == FITRE_CNN_ACT_SWISH) {   // the choice once, not per element
 #pragma unroll
-            for (int i = 0; i < 64; ++i) u[i] *= act_value(p.act, g[i]);
+                for (int i = 0; i < 64; ++i) u[i] *= act_value(FITRE_CNN_ACT_SWISH, g[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 64; ++i) u[i] *= act_value(p.act, g[i]);
+            }
             st.put(p.h, row0, first + c, 0, u);
         }
     }

@@ -241,7 +241,8 @@ token_logprobs_kernel(const T *__restrict__ logits, long ld, const long long *__
     constexpr int LISTS = WARPS > kMaxParts ? WARPS : kMaxParts;
     __shared__ Stats<A> wstat[WARPS];
     __shared__ Stats<A> bstat;                     // this block's part of the row, read by the cluster
-    __shared__ A wbound[WARPS];
+    constexpr int PICK = (kMaxTop + WARPS - 1) / WARPS + 1;   // maxima a warp may put forward
+    __shared__ A picks[TOP ? WARPS * PICK : 1];
     __shared__ int hot[TOP ? THREADS : 1], hots, found;
     __shared__ Entry<A> room[TOP ? kRoom : 1], lists[TOP ? LISTS * kMaxTop : 1], blist[TOP ? kMaxTop : 1];
     cg::cluster_group cluster = cg::this_cluster();
@@ -310,15 +311,15 @@ token_logprobs_kernel(const T *__restrict__ logits, long ld, const long long *__
     }
     if (lane == 0) wstat[warp] = st;
     if (TOP) {
-        // the q-th largest of each warp's maxima, q = top / WARPS rounded up: the smallest of these has at least
-        // `top` elements at or above it
-        A best = run.top, b = best;
-        for (int q = 0; q < (top + WARPS - 1) / WARPS; ++q) {
-            b = warp_max(best);
+        // each warp puts forward its largest maxima, one more than an even share of `top`
+        A best = run.top;
+        const int pick = (top + WARPS - 1) / WARPS + 1;
+        for (int q = 0; q < pick; ++q) {
+            const A b = warp_max(best);
             const unsigned who = __ballot_sync(0xffffffffu, best == b);
             if (lane == __ffs(who) - 1) best = -N::inf();
+            if (lane == 0) picks[warp * pick + q] = b;
         }
-        if (lane == 0) wbound[warp] = b;
         if (tid == 0) hots = found = 0;
         if (tid < kMaxTop) blist[tid] = Entry<A>{-N::inf(), kNone};
     }
@@ -330,9 +331,17 @@ token_logprobs_kernel(const T *__restrict__ logits, long ld, const long long *__
         bstat = r;
     }
     if (TOP) {
-        A bound = wbound[0];
-#pragma unroll
-        for (int w = 1; w < WARPS; ++w) bound = bound < wbound[w] ? bound : wbound[w];
+        // the bound: the top-th largest of what was put forward (every warp finds it for itself)
+        const int n = WARPS * ((top + WARPS - 1) / WARPS + 1);
+        A bound = -N::inf();
+        for (int i0 = 0; i0 < n; i0 += 32) {
+            const int i = i0 + lane;
+            const A v = i < n ? picks[i] : -N::inf();
+            int rank = i < n ? 0 : n;
+            for (int o = 0; o < n; ++o) rank += better(picks[o], o, v, i) ? 1 : 0;
+            const unsigned who = __ballot_sync(0xffffffffu, rank == top - 1);
+            if (who) bound = __shfl_sync(0xffffffffu, v, __ffs(who) - 1);
+        }
         if (run.top >= bound) hot[atomicAdd(&hots, 1)] = tid;   // any order: entries are ranked by value and place
         const bool edge = tid < edges;
         const int edge_at = tid < head ? lo + tid : tail0 + (tid - head);
@@ -340,22 +349,32 @@ token_logprobs_kernel(const T *__restrict__ logits, long ld, const long long *__
         if (edge_v != edge_v) edge_v = -N::inf();               // a NaN ranks as -inf
         if (edge && edge_v >= bound) room[atomicAdd(&found, 1)] = Entry<A>{edge_v, edge_at};
         __syncthreads();
-        // vectors of the hot threads, in rising order of place
+        // the hot threads' vectors: up to 32 of one thread's, or all of several threads', per warp and step
         const int rounds = (nvec + THREADS - 1) / THREADS, hotn = hots;
+        const int wide = rounds >= 32 ? 5 : 32 - __clz(rounds > 1 ? rounds - 1 : 0);   // lanes per thread: 2^wide
         auto each = [&](auto &&use) {
-            for (int i0 = warp * 32; i0 < rounds * hotn; i0 += THREADS) {
-                const int i = i0 + lane, j = i / hotn;
-                const int vec = j < rounds ? hot[i - j * hotn] + j * THREADS : nvec;
-                const bool in = vec < nvec;
-                Vec<T, VEC> raw;
-                if (in) raw = load_vec<T, VEC>(xv + (long)vec * VEC);
-                const bool worth = in && (vec_max(raw) >= bound || bound == -N::inf());
-                if (__any_sync(0xffffffffu, worth))
+            for (int h0 = warp << (5 - wide); h0 < hotn; h0 += WARPS << (5 - wide)) {
+                const int h = h0 + (lane >> wide);
+                const int owner = h < hotn ? hot[h] : nvec;
+                for (int j0 = 0; j0 < rounds; j0 += 2 << wide) {
+                    Vec<T, VEC> raw[2];
+                    int vec[2];
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    A v = worth ? to_acc<A>(raw.v[e]) : -N::inf();
-                    if (v != v) v = -N::inf();
-                    use(worth && v >= bound, v, vbase + vec * VEC + e);
+                    for (int k = 0; k < 2; ++k) {
+                        vec[k] = owner + (j0 + (k << wide) + (lane & ((1 << wide) - 1))) * THREADS;
+                        if (vec[k] < nvec) raw[k] = load_vec<T, VEC>(xv + (long)vec[k] * VEC);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const bool worth = vec[k] < nvec && (vec_max(raw[k]) >= bound || bound == -N::inf());
+                        if (__any_sync(0xffffffffu, worth))
+#pragma unroll
+                            for (int e = 0; e < VEC; ++e) {
+                                A v = worth ? to_acc<A>(raw[k].v[e]) : -N::inf();
+                                if (v != v) v = -N::inf();
+                                use(worth && v >= bound, v, vbase + vec[k] * VEC + e);
+                            }
+                    }
                 }
             }
         };
@@ -374,7 +393,7 @@ token_logprobs_kernel(const T *__restrict__ logits, long ld, const long long *__
                 if (rank < top) blist[rank] = e;
             }
         } else {
-            // too many equal values: sorted lists, in which a later equal value displaces nothing
+            // too many equal values: sorted lists
             WarpList<A> list(top, lane);
             if (warp == 0) list.offer(edge && edge_v >= bound, edge_v, edge_at);
             each([&](bool has, A v, int i) { list.offer(has, v, i); });

@@ -21,7 +21,11 @@
 namespace fitre {
 namespace {
 
-constexpr int N_ELEMS = 16;   // elements of a row one thread holds
+// Elements of a row one thread holds, and the most threads that share a row: fp64 elements take twice the
+// registers, of which 1024 threads have 64 each.
+constexpr int N_ELEMS = 16;
+template <class T> constexpr int n_elems = sizeof(T) == 8 ? 8 : N_ELEMS;
+template <class T> constexpr int max_group = sizeof(T) == 8 ? 512 : 1024;
 
 // Sums `a` and `b` over the G threads of a row; every thread gets the result, added in one fixed
 // order.  `slot` alternates between two halves of the buffer so that one barrier per call suffices.
@@ -185,7 +189,7 @@ __global__ void __launch_bounds__(G, (sizeof(T) == 8 ? 512 : 1024) / G > 0 ? (si
 layer_norm_kernel(const T *x, long ldx, const W *__restrict__ gamma, const W *__restrict__ beta, T *y, long ldy,
                   acc_t<T> *mean, acc_t<T> *rstd, long rows, int cols, double eps) {
     using A = acc_t<T>;
-    constexpr int CH = N_ELEMS / VEC;
+    constexpr int CH = n_elems<T> / VEC;
     __shared__ A buf[4 * (G / 32)];
     const int t = threadIdx.x;
     const A over = A(1) / (A)cols;
@@ -261,7 +265,7 @@ __global__ void __launch_bounds__(G, 1024 / G)
 layer_norm_ring_kernel(const T *x, long ldx, const W *__restrict__ gamma, const W *__restrict__ beta, T *y, long ldy,
                        acc_t<T> *mean, acc_t<T> *rstd, long rows, int cols, double eps, int stages, int *err) {
     using A = acc_t<T>;
-    constexpr int CH = N_ELEMS / VEC;
+    constexpr int CH = n_elems<T> / VEC;
     extern __shared__ __align__(16) unsigned char ring_raw[];
     __shared__ unsigned long long bars[kRingMax];
     __shared__ A buf[4 * (G / 32)];
@@ -411,7 +415,7 @@ layer_norm_backward_kernel(const T *dy, long lddy, const T *x, long ldx, const W
                            const acc_t<T> *__restrict__ mean, const acc_t<T> *__restrict__ rstd, T *dx, long lddx,
                            acc_t<T> *partial, long rows, int cols) {
     using A = acc_t<T>;
-    constexpr int CH = N_ELEMS / VEC;
+    constexpr int CH = n_elems<T> / VEC;
     constexpr int RPB = norm_threads<G> / G;   // rows a block works on at a time
     __shared__ A buf[G > 32 ? 4 * (G / 32) : 1];
     const int t = threadIdx.x % G, group = threadIdx.x / G;
@@ -454,7 +458,7 @@ layer_norm_backward_kernel(const T *dy, long lddy, const T *x, long ldx, const W
         return;
     }
     // the block's warps hold the same columns: added in warp order through shared memory
-    __shared__ A sg[G == 32 ? G * N_ELEMS : 1], sb[G == 32 ? G * N_ELEMS : 1];
+    __shared__ A sg[G == 32 ? G * n_elems<T> : 1], sb[G == 32 ? G * n_elems<T> : 1];
     for (int w = 0; w < RPB; ++w) {
         if (group == w) {
 #pragma unroll
@@ -482,7 +486,7 @@ layer_norm_backward_kernel(const T *dy, long lddy, const T *x, long ldx, const W
 // Rows on 16-byte boundaries through a ring, R (1 or 2) rows at a time: two rows share one barrier and hide one
 // another's latencies.  Elements are read from shared memory twice, for the sums and for dx, so that they need no
 // registers while the block waits for the sums.
-constexpr int kRingThreads = 512;   // resident threads per SM
+constexpr int kRingThreads = 512;   // resident threads per SM of the backward kernels
 template <class T, class W, int VEC, int G, int R>
 __global__ void __launch_bounds__(G, kRingThreads / G > 0 ? kRingThreads / G : 1)
 layer_norm_backward_ring_kernel(const T *dy, long lddy, const T *x, long ldx, const W *__restrict__ gamma,
@@ -490,7 +494,7 @@ layer_norm_backward_ring_kernel(const T *dy, long lddy, const T *x, long ldx, co
                                 acc_t<T> *partial, long rows, int cols, int stages, int *err) {
     using A = acc_t<T>;
     using P = SimdOf<T, VEC>;
-    constexpr int CH = N_ELEMS / VEC, PV = VEC / kPack<VEC>;
+    constexpr int CH = n_elems<T> / VEC, PV = VEC / kPack<VEC>;
     extern __shared__ __align__(16) unsigned char ring_raw[];
     __shared__ unsigned long long bars[kRingMax];
     __shared__ A buf[4 * R * (G / 32)];
@@ -683,9 +687,10 @@ layer_norm_reduce_kernel(const A *__restrict__ partial, int blocks, int cols, W 
     }
 }
 
-int group_for(int cols) {
+// Threads per row; 0: too long for registers.
+int group_for(int cols, bool f64) {
     for (int g : {32, 128, 256, 512, 1024})
-        if (cols <= g * N_ELEMS) return g;
+        if (cols <= g * (f64 ? n_elems<double> : N_ELEMS) && (!f64 || g <= max_group<double>)) return g;
     return 0;
 }
 int blocks_for(long rows, int g, int threads_per_sm) {
@@ -694,7 +699,6 @@ int blocks_for(long rows, int g, int threads_per_sm) {
     const long room = (long)kLmSms * (threads_per_sm > threads ? threads_per_sm / threads : 1);
     return (int)(need < room ? need : room);
 }
-constexpr int kBackThreads = 512;        // resident threads per SM of the backward kernels (128 registers each)
 // Stages of a ring: as many rows as fit the block's share of 200 KB, at least 2 and at most 8 (0: too wide).
 int ring_stages(int threads, int threads_per_sm, long bytes) {
     const int blocks = threads_per_sm / threads > 0 ? threads_per_sm / threads : 1;
@@ -709,7 +713,7 @@ constexpr int kLongSplit = 64;           // row splits of the column sums of lon
 template <class T, class W, int VEC, bool AFFINE>
 void forward_with(fitre_context *ctx, const NormArgs &a) {
     using A = acc_t<T>;
-    const int g = group_for(a.cols);
+    const int g = group_for(a.cols, sizeof(T) == 8);
     const T *x = (const T *)a.x;
     T *y = (T *)a.y;
     const W *gm = (const W *)a.gamma, *bt = (const W *)a.beta;
@@ -738,7 +742,9 @@ void forward_with(fitre_context *ctx, const NormArgs &a) {
             case 128: NORM_LAUNCH(128); break;
             case 256: NORM_LAUNCH(256); break;
             case 512: NORM_LAUNCH(512); break;
-            default: NORM_LAUNCH(1024); break;
+            default:
+                if constexpr (max_group<T> >= 1024) { NORM_LAUNCH(1024); }
+                break;
         }
 #undef NORM_LAUNCH
         check_launch(ctx, "layer_norm_ring_kernel");
@@ -751,7 +757,9 @@ void forward_with(fitre_context *ctx, const NormArgs &a) {
         case 128: NORM_LAUNCH(128); break;
         case 256: NORM_LAUNCH(256); break;
         case 512: NORM_LAUNCH(512); break;
-        case 1024: NORM_LAUNCH(1024); break;
+        case 1024:
+            if constexpr (max_group<T> >= 1024) NORM_LAUNCH(1024);
+            break;
         default:
             layer_norm_long_kernel<T, W><<<blocks, 1024, 0, ctx->stream>>>(x, a.ldx, gm, bt, y, a.ldy, mean, rstd,
                                                                             a.rows, a.cols, a.eps);
@@ -770,13 +778,13 @@ void forward_as(fitre_context *ctx, const NormArgs &a) {
 template <class T, class W, int VEC>
 void backward_as(fitre_context *ctx, const NormArgs &a) {
     using A = acc_t<T>;
-    const int g = group_for(a.cols);
+    const int g = group_for(a.cols, sizeof(T) == 8);
     const T *x = (const T *)a.x, *dy = (const T *)a.dy;
     T *dx = (T *)a.dx;
     const W *gm = (const W *)a.gamma;
     const A *mean = (const A *)a.mean, *rstd = (const A *)a.rstd;
     A *partial = a.dgamma || a.dbeta ? (A *)a.scratch : nullptr;
-    int blocks = blocks_for(a.rows, g ? g : 1024, kBackThreads);
+    int blocks = blocks_for(a.rows, g ? g : 1024, kRingThreads);
     const long bytes = 2l * a.cols * sizeof(T);
     // two rows at a time where three stages of them fit (not in rows above 8192 elements), else one
     const int two = VEC > 1 && g > 32 && g < 1024 ? ring_stages(g, kRingThreads, 2 * bytes) : 0;
@@ -798,7 +806,7 @@ void backward_as(fitre_context *ctx, const NormArgs &a) {
             if (g == 128) NORM_LAUNCH(128, 1);
             else if (g == 256) NORM_LAUNCH(256, 1);
             else if (g == 512) NORM_LAUNCH(512, 1);
-            else NORM_LAUNCH(1024, 1);
+            else if constexpr (max_group<T> >= 1024) NORM_LAUNCH(1024, 1);
         }
 #undef NORM_LAUNCH
         check_launch(ctx, "layer_norm_backward_ring_kernel");
@@ -812,7 +820,9 @@ void backward_as(fitre_context *ctx, const NormArgs &a) {
         case 128: NORM_LAUNCH(128); break;
         case 256: NORM_LAUNCH(256); break;
         case 512: NORM_LAUNCH(512); break;
-        case 1024: NORM_LAUNCH(1024); break;
+        case 1024:
+            if constexpr (max_group<T> >= 1024) NORM_LAUNCH(1024);
+            break;
         default: {
             if (partial) {   // before dx, which may overwrite dy or x
                 const int split = (int)(a.rows < kLongSplit ? a.rows : kLongSplit);
@@ -875,9 +885,15 @@ void norm_dispatch(fitre_context *ctx, const NormArgs &a, bool back) {
 }  // namespace
 
 long layer_norm_backward_scratch(long rows, long cols) {
-    const int g = cols <= 1024 * N_ELEMS ? group_for((int)cols) : 0;
-    const long parts = g ? blocks_for(rows, g, kRingThreads) : (rows < kLongSplit ? rows : kLongSplit);
-    return parts * 2 * cols * (long)sizeof(double);
+    // the larger of what fp64 tensors and the others need
+    long most = 0;
+    for (const bool f64 : {false, true}) {
+        const int g = cols <= 1024 * N_ELEMS ? group_for((int)cols, f64) : 0;
+        const long parts = g ? blocks_for(rows, g, kRingThreads) : (rows < kLongSplit ? rows : kLongSplit);
+        const long bytes = parts * 2 * cols * (f64 ? 8 : 4);
+        most = bytes > most ? bytes : most;
+    }
+    return most;
 }
 void layer_norm_forward(fitre_context *ctx, const NormArgs &a) { norm_dispatch(ctx, a, false); }
 void layer_norm_backward(fitre_context *ctx, const NormArgs &a) { norm_dispatch(ctx, a, true); }
