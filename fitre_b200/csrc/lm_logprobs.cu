@@ -231,7 +231,7 @@ constexpr int kMaxParts = 16;    // blocks that may share a row
 constexpr int kRoom = 256;       // candidates a block can rank at once
 
 template <class T, int THREADS, bool TOP>
-__global__ void __launch_bounds__(THREADS, (sizeof(T) == 8 ? 512 : 768) / THREADS)
+__global__ void __launch_bounds__(THREADS, (sizeof(T) == 8 ? 512 : 1024) / THREADS)
 token_logprobs_kernel(const T *__restrict__ logits, long ld, const long long *__restrict__ tokens, int vocab, int top,
                       acc_t<T> *logprobs, acc_t<T> *lse_out, acc_t<T> *entropy, acc_t<T> *top_logprobs,
                       long long *top_tokens) {
