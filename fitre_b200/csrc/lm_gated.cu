@@ -161,12 +161,26 @@ gated_slopes_kernel(const T *dh, long lddh, const T *g, long ldg, const T *u, lo
     store_vec<T, VEC>(out + half + row * ld + at, du);
 }
 
-// A matrix whose rows TMA cannot read, copied to rows that it can, padded with zeros.
+// Matrices whose rows TMA cannot read, copied to rows that it can, padded with zeros: a warp per row.
+template <class T> struct Copies {
+    const T *in[3];
+    T *out[3];
+    long ld[3], rows[3];
+};
 template <class T>
 __global__ void __launch_bounds__(256)
-align_rows_kernel(const T *in, long ld, T *out, long ldo, long rows, int cols) {
-    for (long row = blockIdx.x; row < rows; row += gridDim.x)
-        for (int c = threadIdx.x; c < ldo; c += 256) out[row * ldo + c] = c < cols ? in[row * ld + c] : from_acc<T>(0.0f);
+align_rows_kernel(Copies<T> k, int cols, int ldo) {
+    wait_for_previous_kernel();
+    let_next_kernel_start();
+    const int lane = threadIdx.x & 31;
+    const long row = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const T *in = k.in[blockIdx.y];
+    T *out = k.out[blockIdx.y];
+    if (row >= k.rows[blockIdx.y]) return;
+    in += row * k.ld[blockIdx.y];
+    out += row * ldo;
+#pragma unroll 4
+    for (int c = lane; c < ldo; c += 32) out[c] = c < cols ? in[c] : from_acc<T>(0.0f);
 }
 
 long up8(long n) { return (n + 7) / 8 * 8; }
@@ -189,17 +203,15 @@ Operands<T> readable(fitre_context *ctx, const GatedArgs &a, char *&room) {
     Operands<T> o{(const T *)a.x, (const T *)a.wg, (const T *)a.wu, a.ldx, a.ldwg, a.ldwu};
     if (a.width % 8 == 0) return o;
     const long ld = up8(a.width);
-    auto copy = [&](const T *in, long ldi, long rows) {
-        T *out = (T *)room;
-        room += up128(2 * rows * ld);
-        align_rows_kernel<T><<<(unsigned)(rows < 16 * kLmSms ? rows : 16 * kLmSms), 256, 0, ctx->stream>>>(
-            in, ldi, out, ld, rows, (int)a.width);
-        check_launch(ctx, "align_rows_kernel");
-        return out;
-    };
-    o.x = copy(o.x, a.ldx, a.tokens);
-    o.wg = copy(o.wg, a.ldwg, a.hidden);
-    o.wu = copy(o.wu, a.ldwu, a.hidden);
+    Copies<T> k = {{o.x, o.wg, o.wu}, {}, {a.ldx, a.ldwg, a.ldwu}, {a.tokens, a.hidden, a.hidden}};
+    for (int i = 0; i < 3; ++i) {
+        k.out[i] = (T *)room;
+        room += up128(2 * k.rows[i] * ld);
+    }
+    const long most = a.tokens > a.hidden ? a.tokens : a.hidden;
+    launch_after(ctx->stream, align_rows_kernel<T>, dim3((unsigned)((most + 7) / 8), 3), 256, k, (int)a.width, (int)ld);
+    check_launch(ctx, "align_rows_kernel");
+    o.x = k.out[0], o.wg = k.out[1], o.wu = k.out[2];
     o.ldx = o.ldwg = o.ldwu = ld;
     return o;
 }
@@ -217,7 +229,7 @@ void forward_tiles(fitre_context *ctx, const GatedArgs &a, const Operands<T> &o)
     g.epi.g = gemm_output<T>(a.g, F, T_, 1, a.ldg, 0, fmt_of<T>);
     g.epi.u = gemm_output<T>(a.u, F, T_, 1, a.ldu, 0, fmt_of<T>);
     g.epi.act = a.act;
-    gemm_launch<CG, BN, false, false, GatedEpi<T>>(ctx, g, T_, F, 1, false, D, 1, fmt_of<T>, "gated_tiles_kernel", false);
+    gemm_launch<CG, BN, false, false, GatedEpi<T>>(ctx, g, T_, F, 1, false, D, 1, fmt_of<T>, "gated_tiles_kernel", a.width % 8 != 0);
 }
 
 // Whether a product has tiles enough for the SM pairs' 256-row tiles; below, 128-row tiles on single SMs
@@ -266,8 +278,7 @@ void input_gradient(fitre_context *ctx, const GatedArgs &a, const Operands<T> &o
     gemm_operand(&g.b[0], true, o.wg, up8(D), F, 1, o.ldwg, 0, fmt_of<T>);
     gemm_operand(&g.b[1], true, o.wu, up8(D), F, 1, o.ldwu, 0, fmt_of<T>);
     g.epi.out[0] = gemm_output<T>(a.dx, D, T_, 1, a.lddx, 0, fmt_of<T>);
-    gemm_launch<CG, BN, false, true, StoreEpi<T>>(ctx, g, T_, D, 1, false, F, 2, fmt_of<T>, "gated_input_gradient_kernel",
-                                                    a.width % 8 == 0);
+    gemm_launch<CG, BN, false, true, StoreEpi<T>>(ctx, g, T_, D, 1, false, F, 2, fmt_of<T>, "gated_input_gradient_kernel", true);
 }
 template <class T, int CG, int BN>
 void weight_gradient(fitre_context *ctx, const GatedArgs &a, const Operands<T> &o, const T *slopes, long ld, long half) {

@@ -15,8 +15,8 @@
 //              columns in shared memory and sends them off as one TMA store: full cache lines, edges clipped.
 // CG = 2 pairs two SMs on a 256 x BN tile: each CTA loads its 128 rows of A and half of B's rows, so a byte
 // of B feeds twice the arithmetic; the even CTA's issuer drives both.  CG = 1 (128 x BN) is for products
-// with too few tiles to occupy the pairs; where even those leave SMs idle, a cluster of 2 or 4 CTAs divides a tile's k
-// among itself and each CTA adds up and stores a part of the tile's rows, from the others' partial sums in its
+// with too few tiles to occupy the pairs; where even those leave SMs idle, a cluster of 2 to 8 CTAs divides a tile's k
+// among itself and each CTA adds up and stores a part of the tile, from the others' partial sums in its
 // shared memory (1003 x 1000 x 5460: 39 -> 18 us against halving the tiles).  Every wait is bounded; when one runs out, the CTA sets the
 // context's error word, lets its copies in flight land, frees its TMEM and returns.
 #pragma once
@@ -221,8 +221,8 @@ struct Stager {
     int lane, turn;
     uint32_t phase;
     bool loading;
-    uint32_t partial;   // other CTAs' sums for this warp's rows, `parts` blocks of [128 columns][32 rows]
-    int parts;
+    uint32_t partial;   // other CTAs' sums for this warp's part of the tile, `parts` blocks of `block` bytes: [columns][32 rows]
+    int parts, block;
     // 64 accumulator columns of this thread's row, the first of them column `c` of the tile at `tmem`
     __device__ __forceinline__ void sums(uint32_t tmem, int c, float (&v)[64]) const {
         tmem_load64(tmem + c, v);
@@ -230,7 +230,7 @@ struct Stager {
 #pragma unroll
             for (int e = 0; e < 64; ++e) {
                 float o;
-                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(o) : "r"(partial + s * 16384 + (c + e) * 128 + lane * 4));
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(o) : "r"(partial + s * block + (c + e) * 128 + lane * 4));
                 v[e] += o;
             }
     }
@@ -526,7 +526,7 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
         if (!ok) *gave_up = 1;
     }
     const int quarter = warp & 3;   // the TMEM lanes an epilogue warp may read
-    Stager stager{smem_u32(sm + ST * L::STAGE) + quarter * 8192, smem_u32(bars + 22 + quarter), gave_up, lane, 0, 0, false, 0, 0};
+    Stager stager{smem_u32(sm + ST * L::STAGE) + quarter * 8192, smem_u32(bars + 22 + quarter), gave_up, lane, 0, 0, false, 0, 0, 0};
     if (warp >= 2 && split == 1) {
         // ---------------- epilogue ----------------
         const uint32_t freed = CG == 2 ? map_to_rank(smem_u32(bars + 18), 0) : smem_u32(bars + 18);
@@ -556,32 +556,41 @@ tile_gemm_kernel(const __grid_constant__ GemmArgs<typename Epi::Params> p) {
         if (!done) *gave_up = 1;
         __syncwarp();
         cluster_barrier();   // every CTA's stages are free
-        const int owner = quarter * split / 4, own = 4 / split;   // who adds up these 32 rows; row quarters per CTA
+        // The tile in parts of 32 rows x `span` columns (all of them, or half for 8 CTAs); owner of part (quarter, h): who
+        // adds it up.  A CTA's parts lie one behind the other in its shared memory, in each the others' sums in turn.
+        const int halves = split == 8 ? 2 : 1, span = BN / halves, block = span * 128;
+        const int per = 4 * halves / split;   // parts per CTA
         const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
-        const uint32_t room = smem_u32(sm) + (quarter % own) * (split - 1) * 16384;
         if (warp >= 2) {
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            if (owner != part) {
-                const uint32_t to = map_to_rank(room + (part < owner ? part : part - 1) * 16384, owner) + lane * 4;
 #pragma unroll 1
-                for (int c = 0; c < BN; c += 64) {
-                    float v[64];
-                    tmem_load64(mine + c, v);
+            for (int c = 0; c < BN; c += 64) {
+                const int piece = quarter * halves + c / span, owner = piece / per;
+                if (owner == part) continue;
+                const uint32_t room = smem_u32(sm) + ((piece % per) * (split - 1) + (part < owner ? part : part - 1)) * block;
+                const uint32_t to = map_to_rank(room, owner) + lane * 4 + (c % span) * 128;
+                float v[64];
+                tmem_load64(mine + c, v);
 #pragma unroll
-                    for (int e = 0; e < 64; ++e)
-                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + (c + e) * 128), "f"(v[e]) : "memory");
-                }
+                for (int e = 0; e < 64; ++e)
+                    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + e * 128), "f"(v[e]) : "memory");
             }
         }
         __syncwarp();
         cluster_barrier();   // the partial sums have arrived
-        if (warp >= 2 && owner == part) {
-            const TileAt at = tile_at(g, first);
+        if (warp >= 2) {
+            TileAt at = tile_at(g, first);
             const int row0 = at.m * 128 + quarter * 32;
-            stager.partial = room;
-            stager.parts = split - 1;
-            Epi::template begin<BN>(p.epi, at, row0, stager);
-            Epi::template store<BN>(p.epi, at, row0, mine, stager);
+            for (int h = 0; h < halves; ++h) {
+                const int piece = quarter * halves + h;
+                if (piece / per != part) continue;
+                if (halves == 2) at.half = h;
+                stager.partial = smem_u32(sm) + (piece % per) * (split - 1) * block;
+                stager.parts = split - 1;
+                stager.block = block;
+                Epi::template begin<BN>(p.epi, at, row0, stager);
+                Epi::template store<BN>(p.epi, at, row0, mine + h * span, stager);
+            }
         }
     }
     if (warp >= 2) {
@@ -697,6 +706,7 @@ void gemm_launch(fitre_context *ctx, GemmArgs<typename Epi::Params> &args, int M
     g.split = 1;
     if (CG == 1 && tiles <= kLmSms / 2 && stages >= 8) {
         g.split = tiles <= kLmSms / 4 && stages >= 16 ? 4 : 2;
+        if (!Epi::kTwoMaps && tiles <= kLmSms / 8 && stages >= 32) g.split = 8;   // two maps: no halves of a tile
         g.whole = tiles;
     }
     g.total = g.whole + 2 * (tiles - g.whole);
