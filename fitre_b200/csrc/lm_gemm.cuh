@@ -17,7 +17,7 @@
 // of B feeds twice the arithmetic; the even CTA's issuer drives both.  CG = 1 (128 x BN) is for products
 // with too few tiles to occupy the pairs; where even those leave SMs idle, a cluster of 2 to 8 CTAs divides a tile's k
 // among itself and each CTA adds up and stores a part of the tile, from the others' partial sums in its
-// shared memory (1003 x 1000 x 5460: 39 -> 18 us against halving the tiles).  Every wait is bounded; when one runs out, the CTA sets the
+// shared memory (1003 x 1000 x 5460: 39 -> 27 us against halving the tiles).  Every wait is bounded; when one runs out, the CTA sets the
 // context's error word, lets its copies in flight land, frees its TMEM and returns.
 #pragma once
 
@@ -701,12 +701,14 @@ void gemm_launch(fitre_context *ctx, GemmArgs<typename Epi::Params> &args, int M
     const int room = kLmSms / CG, tiles = (int)per * batch, left = tiles % room;
     // (64 columns are the least an epilogue stores at a time; two maps on one SM load no half tiles)
     g.whole = left > 0 && left <= room / 2 && !(Epi::kTwoMaps && CG == 1) ? tiles - left : tiles;
-    // dividing k is worth its exchange of partial sums from a few stages per CTA on
+    // Dividing k costs an exchange of about 3 us, as much as 6 stages: worth it for long sums only (five steps
+    // of a 1024 x 1024 update, 8 stages a product: 148 us in halves, 196 us divided by 2; 1003 x 1000 x 5460, 44 stages: 39
+    // us in halves, 27 us divided by 2).
     const int stages = (int)((K + G_KB - 1) / G_KB) * nseg;
     g.split = 1;
-    if (CG == 1 && tiles <= kLmSms / 2 && stages >= 8) {
-        g.split = tiles <= kLmSms / 4 && stages >= 16 ? 4 : 2;
-        if (!Epi::kTwoMaps && tiles <= kLmSms / 8 && stages >= 32) g.split = 8;   // two maps: no halves of a tile
+    if (CG == 1 && tiles <= kLmSms / 2 && stages >= 24) {
+        g.split = tiles <= kLmSms / 4 && stages >= 32 ? 4 : 2;
+        if (!Epi::kTwoMaps && tiles <= kLmSms / 8 && stages >= 64) g.split = 8;   // two maps: no halves of a tile
         g.whole = tiles;
     }
     g.total = g.whole + 2 * (tiles - g.whole);
