@@ -701,15 +701,19 @@ void gemm_launch(fitre_context *ctx, GemmArgs<typename Epi::Params> &args, int M
     const int room = kLmSms / CG, tiles = (int)per * batch, left = tiles % room;
     // (64 columns are the least an epilogue stores at a time; two maps on one SM load no half tiles)
     g.whole = left > 0 && left <= room / 2 && !(Epi::kTwoMaps && CG == 1) ? tiles - left : tiles;
-    // Dividing k costs an exchange of about 3 us, as much as 6 stages: worth it for long sums only (five steps
-    // of a 1024 x 1024 update, 8 stages a product: 148 us in halves, 196 us divided by 2; 1003 x 1000 x 5460, 44 stages: 39
+    // Dividing k by S costs an exchange worth about 5 + S / 2 stages of 0.5 us: for long sums only (five steps of a
+    // 1024 x 1024 update, 8 stages a product: 148 us in halves, 196 us divided by 2; 1003 x 1000 x 5460, 44 stages: 39
     // us in halves, 27 us divided by 2).
     const int stages = (int)((K + G_KB - 1) / G_KB) * nseg;
     g.split = 1;
-    if (CG == 1 && tiles <= kLmSms / 2 && stages >= 24) {
-        g.split = tiles <= kLmSms / 4 && stages >= 32 ? 4 : 2;
-        if (!Epi::kTwoMaps && tiles <= kLmSms / 8 && stages >= 64) g.split = 8;   // two maps: no halves of a tile
-        g.whole = tiles;
+    if (CG == 1) {
+        int best = stages;
+        for (int s : {2, 4, 8}) {
+            const int cost = (stages + s - 1) / s + 5 + s / 2;
+            // eight CTAs share a tile by its column halves, which two maps on one SM do not have
+            if (tiles * s <= kLmSms && cost < best && !(s == 8 && Epi::kTwoMaps)) best = cost, g.split = s;
+        }
+        if (g.split > 1) g.whole = tiles;
     }
     g.total = g.whole + 2 * (tiles - g.whole);
     g.triangle = triangle;
