@@ -35,18 +35,25 @@ __device__ __forceinline__ double block_sum(double q, double *s) {
     return q;
 }
 
-// Sums of squares of each matrix's parts, in fp64 (squares of fp32 values overflow fp32): part p holds every
-// gridDim.x-th row.
+// Threads of a block that share a row of `chunks` vectors: a power of two from 8 to 256, as its logarithm.
+inline int row_share(long chunks) {
+    int s = 3;
+    while (s < 8 && (1 << s) < chunks) ++s;
+    return s;
+}
+// Sums of squares of each matrix's parts, in fp64 (squares of fp32 values overflow fp32): the blocks of a matrix take
+// 256 >> share rows at a time in turn.
 template <class T, int VEC>
 __global__ void __launch_bounds__(256)
-ortho_norm_kernel(const T *in, long ld, long bstride, int rows, int cols, double *partial) {
+ortho_norm_kernel(const T *in, long ld, long bstride, int rows, int cols, int share, double *partial) {
     let_next_kernel_start();
     __shared__ double s[8];
     const T *m = in + blockIdx.y * bstride;
+    const int t = threadIdx.x & ((1 << share) - 1), at = threadIdx.x >> share, step = 256 >> share;
     double q = 0;
-    for (int r = blockIdx.x; r < rows; r += gridDim.x)
+    for (int r = blockIdx.x * step + at; r < rows; r += gridDim.x * step)
 #pragma unroll 4
-        for (int c = threadIdx.x * VEC; c < cols; c += 256 * VEC) {
+        for (int c = t * VEC; c < cols; c += VEC << share) {
             const Vec<T, VEC> x = load_vec<T, VEC>(m + r * ld + c);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
@@ -61,8 +68,8 @@ ortho_norm_kernel(const T *in, long ld, long bstride, int rows, int cols, double
 // The first iterate, as a pair of fp16 matrices; zeros in the padding of their rows.
 template <class T, int VEC>
 __global__ void __launch_bounds__(256)
-ortho_scale_kernel(const T *in, long ld, long bstride, int rows, int cols, const double *__restrict__ partial, int parts,
-                   double eps, __half *hi, __half *lo, long ldo, long ostride) {
+ortho_scale_kernel(const T *in, long ld, long bstride, int rows, int cols, int share, const double *__restrict__ partial,
+                   int parts, double eps, __half *hi, __half *lo, long ldo, long ostride) {
     wait_for_previous_kernel();
     let_next_kernel_start();
     __shared__ double s[8];
@@ -72,9 +79,10 @@ ortho_scale_kernel(const T *in, long ld, long bstride, int rows, int cols, const
     const T *m = in + blockIdx.y * bstride;
     hi += blockIdx.y * ostride;
     lo += blockIdx.y * ostride;
-    for (int r = blockIdx.x; r < rows; r += gridDim.x)
+    const int t = threadIdx.x & ((1 << share) - 1), at = threadIdx.x >> share, step = 256 >> share;
+    for (int r = blockIdx.x * step + at; r < rows; r += gridDim.x * step) {
 #pragma unroll 2
-        for (int c = threadIdx.x * VEC; c < cols; c += 256 * VEC) {
+        for (int c = t * VEC; c < cols; c += VEC << share) {
             const Vec<T, VEC> x = load_vec<T, VEC>(m + r * ld + c);
             Vec<__half, VEC> h, l;
 #pragma unroll
@@ -86,8 +94,8 @@ ortho_scale_kernel(const T *in, long ld, long bstride, int rows, int cols, const
             store_vec<__half, VEC>(hi + r * ldo + c, h);
             store_vec<__half, VEC>(lo + r * ldo + c, l);
         }
-    for (int r = blockIdx.x; r < rows; r += gridDim.x)
-        if (cols + (int)threadIdx.x < ldo) hi[r * ldo + cols + threadIdx.x] = lo[r * ldo + cols + threadIdx.x] = __float2half_rn(0.0f);
+        if (cols + t < ldo) hi[r * ldo + cols + t] = lo[r * ldo + cols + t] = __float2half_rn(0.0f);   // fewer than 8
+    }
 }
 
 // A symmetric product: tile and, off the diagonal, its mirror image.  out = kacc * acc + kin * in; with
@@ -182,10 +190,13 @@ struct IterateEpi {
         if (row0 >= p.out.rows) return;
         const float *diag = p.diag + (long)at.batch * p.small;
         const float drow = !p.tall && row < p.out.rows ? diag[row] : 0.0f;
+        // tall: the diagonal runs along the columns; each lane holds two of the block's 64 and passes them round
+        auto along = [&](int col) { return p.tall && col + st.lane < p.cols ? diag[col + st.lane] : 0.0f; };
+        float d0 = along(first), d1 = along(first + 32);
         const P kacc = P::splat(p.kacc), kout = P::splat(p.kout), a = P::splat(p.a), minus = P::splat(-1.0f);
 #pragma unroll 1
         for (int c = 0; c < width && first + c < p.out.cols; c += 64) {
-            const int col = first + c, left = p.cols - col;
+            const int col = first + c;
             float acc[64];
             st.sums(tmem, c, acc);
             st.wait();
@@ -200,7 +211,10 @@ struct IterateEpi {
                     const int e = i * 8 + j * 2;
                     const float2 fh = unpack_half2(h[j]), fl = unpack_half2(l[j]);
                     P ad = P::splat(p.a + drow);
-                    if (p.tall) ad = add(a, P::of(e < left ? diag[col + e] : 0.0f, e + 1 < left ? diag[col + e + 1] : 0.0f));
+                    if (p.tall) {
+                        const float d = e < 32 ? d0 : d1;
+                        ad = add(a, P::of(__shfl_sync(0xffffffffu, d, e & 31), __shfl_sync(0xffffffffu, d, (e + 1) & 31)));
+                    }
                     P x = fma(P::of(fl.x, fl.y), kLast ? ad : a, mul(P::of(fh.x, fh.y), ad));
                     x = fma(P::of(acc[e], acc[e + 1]), kacc, mul(x, kout));
                     float x0, x1;
@@ -213,6 +227,8 @@ struct IterateEpi {
                     }
                 }
             }
+            d0 = along(col + 64);
+            d1 = along(col + 96);
             __syncwarp();
             st.put(p.out, row0, col, at.batch, w);
             if constexpr (!kLast) st.put(p.lo, row0, col, at.batch, r);
@@ -309,11 +325,12 @@ void iterate(fitre_context *ctx, const Plan &pl, const __half *x, T *out, long l
 template <class T, int VEC>
 void start_as(fitre_context *ctx, const OrthoArgs &a, const Plan &pl) {
     const dim3 grid(pl.parts, pl.batch);
+    const int share = row_share((pl.cols + VEC - 1) / VEC);
     ortho_norm_kernel<T, VEC><<<grid, 256, 0, ctx->stream>>>((const T *)a.in, a.ldi, a.istride, pl.rows, pl.cols,
-                                                             pl.partial);
+                                                             share, pl.partial);
     check_launch(ctx, "ortho_norm_kernel");
     launch_after(ctx->stream, ortho_scale_kernel<T, VEC>, grid, 256, (const T *)a.in, a.ldi, a.istride, pl.rows, pl.cols,
-                 pl.partial, pl.parts, a.eps, pl.x[0], pl.lo, pl.ldx, pl.xs);
+                 share, pl.partial, pl.parts, a.eps, pl.x[0], pl.lo, pl.ldx, pl.xs);
     check_launch(ctx, "ortho_scale_kernel");
 }
 template <class T>
