@@ -64,7 +64,8 @@ void need_norm_shape(int dtype, int wtype, long rows, long cols) {
     FITRE_REQUIRE(wtype == dtype || (wtype == FITRE_DTYPE_F32 && dtype != FITRE_DTYPE_F64), FITRE_ERR_UNSUPPORTED,
                   "layer norm: weights are of the tensor's type, or fp32 next to a 16-bit one");
     need(rows >= 0 && cols >= 1, "layer norm: rows >= 0 and cols >= 1");
-    FITRE_REQUIRE(cols <= (1l << 28) && rows <= (1l << 40), FITRE_ERR_TOO_LARGE, "layer norm: too large");
+    FITRE_REQUIRE(cols <= (1l << 28) && rows <= (1l << 33), FITRE_ERR_TOO_LARGE,
+                  "layer norm: at most 2^33 rows of 2^28 elements");
 }
 void need_token_shape(int dtype, long rows, long vocab) {
     need_type(dtype);

@@ -705,10 +705,16 @@ int ring_stages(int threads, int threads_per_sm, long bytes) {
     const long s = 200 * 1024 / blocks / bytes;
     return s < 2 ? 0 : s > kRingMax ? kRingMax : (int)s;
 }
-template <class K> void allow_shared(K kernel, size_t bytes) {
-    FITRE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-}
 constexpr int kLongSplit = 64;           // row splits of the column sums of long rows
+// Lets a kernel use `bytes` of dynamic shared memory (asked for once per device and thread while it is enough).
+template <auto kernel> void allow_shared(const fitre_context *ctx, long bytes) {
+    static thread_local int device = -1;
+    static thread_local long allowed = 0;
+    if (device == ctx->device && bytes <= allowed) return;
+    FITRE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    device = ctx->device;
+    allowed = bytes;
+}
 
 template <class T, class W, int VEC, bool AFFINE>
 void forward_with(fitre_context *ctx, const NormArgs &a) {
@@ -735,7 +741,7 @@ void forward_with(fitre_context *ctx, const NormArgs &a) {
     if constexpr (VEC > 1) if (stages) {
         const int room = blocks_for(a.rows, g, 1024);
 #define NORM_LAUNCH(G)                                                                                       \
-    allow_shared(layer_norm_ring_kernel<T, W, VEC, G, AFFINE>, stages * bytes);                                      \
+    allow_shared<layer_norm_ring_kernel<T, W, VEC, G, AFFINE>>(ctx, stages * bytes);                                      \
     layer_norm_ring_kernel<T, W, VEC, G, AFFINE><<<room, G, stages * bytes, ctx->stream>>>(                          \
         x, a.ldx, gm, bt, y, a.ldy, mean, rstd, a.rows, a.cols, a.eps, stages, (int *)(ctx->dscal + 4000))
         switch (g) {
@@ -793,7 +799,7 @@ void backward_as(fitre_context *ctx, const NormArgs &a) {
         blocks = blocks_for(a.rows, g, kRingThreads);
 #define NORM_LAUNCH(G, R)                                                                                    \
     do {                                                                                                     \
-        allow_shared(layer_norm_backward_ring_kernel<T, W, VEC, G, R>, stages * R * bytes);                  \
+        allow_shared<layer_norm_backward_ring_kernel<T, W, VEC, G, R>>(ctx, stages * R * bytes);                  \
         layer_norm_backward_ring_kernel<T, W, VEC, G, R><<<blocks, G, stages * R * bytes, ctx->stream>>>(    \
             dy, a.lddy, x, a.ldx, gm, mean, rstd, dx, a.lddx, partial, a.rows, a.cols, stages,               \
             (int *)(ctx->dscal + 4000));                                                                     \

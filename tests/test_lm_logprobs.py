@@ -11,7 +11,7 @@ from fitre_b200 import api
 gpu = pytest.mark.gpu
 INF = float("inf")
 SHAPES = [(1, 1), (2, 5), (3, 33), (1, 4097), (300, 130), (2, 8193), (1, 50001), (5, 32000), (160, 5000), (1, 131072),
-          (2, 256000)]
+          (2, 256000), (200, 70001), (1500, 4096)]
 
 
 def reference(x, tokens, top):
@@ -266,3 +266,26 @@ def test_refusals_and_no_rows():
     refused(S.ERR_BAD_ARG, b, c, x, t, s, s, s, None, x[:, :39])
     f(c, x[:0], t[:0], s[:0])
     b(c, x[:0], t[:0], s[:0], None, s[:0], None, x[:0])
+
+
+@gpu
+def test_two_streams_at_once():
+    """Contexts of their own on two streams: nothing is shared between them."""
+    g = U.gen(9)
+    xs = [U.randn(g, 120, 30000, dtype=torch.bfloat16, scale=3.0) for _ in range(2)]
+    tok = torch.zeros(120, device="cuda", dtype=torch.int64)
+    alone = [outputs(120, 8, torch.bfloat16) for _ in xs]
+    for x, o in zip(xs, alone):
+        api.tokenLogProbs(U.ctx(), x, tok, *o)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    ctxs = [U.ctx(s) for s in streams]
+    both = [outputs(120, 8, torch.bfloat16) for _ in xs]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for c, x, o in zip(ctxs, xs, both):
+            api.tokenLogProbs(c, x, tok, *o)
+    for c in ctxs:
+        c.synchronize()
+    for a, b in zip(alone, both):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))

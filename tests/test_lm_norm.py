@@ -10,7 +10,8 @@ from fitre_b200 import api
 
 gpu = pytest.mark.gpu
 SHAPES = [(1, 1), (3, 7), (5, 32), (4, 512), (9, 513), (2, 1000), (3, 2048), (600, 2049), (7, 4096), (2, 8191),
-          (3, 8192), (2, 16384), (2, 16385), (70, 20011), (1501, 96), (4001, 257)]
+          (3, 8192), (2, 16384), (2, 16385), (70, 20011), (1501, 96), (4001, 257), (2001, 1536), (1300, 4096), (901, 8192),
+          (451, 9176)]
 
 
 def reference(x, gamma, beta, eps):

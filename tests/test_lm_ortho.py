@@ -56,7 +56,7 @@ BOUND = 4.1e-3
 
 @gpu
 @pytest.mark.parametrize("shape", [(1, 1, 1), (2, 1, 40), (1, 17, 5), (3, 8, 8), (1, 64, 64), (2, 100, 260), (1, 129, 128),
-                                   (5, 513, 384), (1, 1000, 77), (2, 384, 1001), (1, 1024, 1024), (1, 300, 4000),
+                                   (5, 513, 384), (1, 1000, 77), (2, 384, 1001), (1, 1024, 1024), (1, 300, 4000), (2, 3000, 200),
                                    (2, 2304, 2560), (2, 2600, 2304)], ids=str)
 @pytest.mark.parametrize("kind", ["full", "low", "mixed"])
 def test_against_the_polynomial(shape, kind):
@@ -237,3 +237,21 @@ def test_one_training_step():
         want = polynomial(grad)
         assert (mine.double() - want).norm() < BOUND * want.norm()
 
+
+
+@gpu
+def test_products_on_two_streams_at_once():
+    """The tensor-core kernels take whole SMs and wait within their clusters only: two streams interleave freely."""
+    gs = [update(2, 300, 520, "mixed", torch.float32, s) for s in (1, 2)]
+    alone = [run(g) for g in gs]
+    streams = [torch.cuda.Stream() for _ in gs]
+    ctxs = [U.ctx(s) for s in streams]
+    outs = [torch.zeros_like(a) for a in alone]
+    scratch = [torch.empty(api.orthogonalizeMemRequired(2, 300, 520), device="cuda", dtype=torch.float64) for _ in gs]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for c, g, o, w in zip(ctxs, gs, outs, scratch):
+            api.orthogonalizeUpdate(c, g, o, w)
+    for c in ctxs:
+        c.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(alone, outs))
