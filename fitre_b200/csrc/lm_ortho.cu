@@ -119,6 +119,8 @@ struct SymmetricEpi {
         const int row = row0 + st.lane, n = p.out.rows;
         const int first = at.n * BN + (at.half > 0 ? BN / 2 : 0), width = at.half < 0 ? BN : BN / 2;
         if (row0 >= n) return;
+        using P = Simd<float, 2>;
+        const P kacc = P::splat(p.kacc), kin = P::splat(p.kin);
 #pragma unroll 1
         for (int c = 0; c < width && first + c < n; c += 64) {
             const int col = first + c;
@@ -126,7 +128,6 @@ struct SymmetricEpi {
             float acc[64];
             st.sums(tmem, c, acc);
             if (p.with_in) st.wait();
-            const int on = p.diag && row < n ? row - col : -1;   // this row's diagonal element in the block, if 0..63
             uint32_t w[32];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -136,14 +137,23 @@ struct SymmetricEpi {
                 for (int j = 0; j < 4; ++j) {
                     const int e = i * 8 + j * 2;
                     const float2 f = unpack_half2(q[j]);
-                    float x = p.kacc * acc[e] + p.kin * f.x, y = p.kacc * acc[e + 1] + p.kin * f.y;
-                    if ((on & ~1) == e) {
-                        p.diag[(long)at.batch * n + row] = (on & 1 ? y : x) * (1 / kScale);
-                        if (on & 1) y = 0.0f;
-                        else x = 0.0f;
-                    }
+                    const P v = fma(P::of(acc[e], acc[e + 1]), kacc, mul(P::of(f.x, f.y), kin));
+                    float x, y;
+                    v.split(x, y);
                     w[i * 4 + j] = pack2<__half>(x, y);
+                    acc[e] = x;
+                    acc[e + 1] = y;
                 }
+            }
+            if (p.diag && row0 < col + 64 && row0 + 32 > col) {   // the diagonal runs through this block
+                const int on = row - col;                         // this row's element, if 0..63
+                float d = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 64; ++e) d = on == e ? acc[e] : d;
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    w[e] &= on >> 1 == e ? (on & 1 ? 0x0000ffffu : 0xffff0000u) : 0xffffffffu;
+                if (row < n && on >= 0 && on < 64) p.diag[(long)at.batch * n + row] = d * (1 / kScale);
             }
             __syncwarp();
             st.put(p.out, row0, col, at.batch, w);
