@@ -4,7 +4,8 @@
  * The library accelerates one path of kylasa/FITRE: the CNN gradient
  * (forward + backward), the exact Hessian-vector product by Pearlmutter's
  * R-operator, the one-direction quadratic model, Steihaug-CG driven by that
- * Hessian-vector product, and KFAC factor accumulation.  Every entry point is
+ * Hessian-vector product, and KFAC factor accumulation.  A section of its own at the
+ * end holds operators for language models.  Every entry point is
  * `extern "C"`, takes plain pointers and sizes, and returns an `int` status
  * (FITRE_OK == 0).  `real` is `double` (reference: core/datadefs.h:5).
  *
