@@ -11,6 +11,9 @@
 // core takes no wider operand next to 16-bit weights), then dx is one product over both halves of the
 // concatenated inner dimension, and dWg / dWu one launch over both.
 // All sums are fp32; each output is rounded once.
+// Measured on a B200: 8192 x 4096 x 12288 bf16 with g and u stored 1089 us from a cool start (1515 TFLOP/s; cuBLAS 1029 us for
+// the two projections without activation, product or their stores), 1240 us in a loop under the power cap;
+// gradient at 4096 tokens 1187 / 1360 us; one token 37 us (5.4 TB/s of weights).
 #include "lm_gemm.cuh"
 #include "lm_simd.cuh"
 

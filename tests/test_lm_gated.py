@@ -246,3 +246,24 @@ def test_refusals():
     refused(S.ERR_WORKSPACE, b, c, h, x, w, w, h, h, x.clone(), w.clone(), w.clone(), devPtr=ws[:4])
     f(c, x, w, w, h)
     c.synchronize()
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    t, d, f, ld = 33000, 64, 72, 70000
+    x, wg, wu, gen = data((t, d, f), torch.bfloat16, 2)
+    far = torch.empty(t * ld, device="cuda", dtype=torch.bfloat16).as_strided((t, d), (ld, 1))
+    far.copy_(x)
+    c = U.ctx()
+    results = []
+    for view in (far, x):
+        h, g, u = (torch.empty(t, f, device="cuda", dtype=torch.bfloat16) for _ in range(3))
+        api.gatedForward(c, view, wg, wu, h, g, u)
+        dx, dwg, dwu = torch.empty_like(x), torch.empty_like(wg), torch.empty_like(wu)
+        api.gatedBackward(c, h, view, wg, wu, g, u, dx, dwg, dwu, SWISH, scratch(api.gatedBackwardMemRequired(t, d, f)))
+        results.append((h, g, u, dx, dwg, dwu))
+    c.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    ws = scratch(api.gatedBackwardMemRequired(t, d, f))
+    api.gatedBackward(c, results[0][0], x, wg, wu, *results[0][1:3], far, torch.empty_like(wg), torch.empty_like(wu), SWISH, ws)
+    assert torch.equal(far, results[0][3])

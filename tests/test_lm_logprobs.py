@@ -289,3 +289,25 @@ def test_two_streams_at_once():
         c.synchronize()
     for a, b in zip(alone, both):
         assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    rows, vocab, ld = 33000, 200, 70000
+    g = U.gen(13)
+    base = torch.empty(rows * ld, device="cuda", dtype=torch.bfloat16)
+    x = base.as_strided((rows, vocab), (ld, 1))
+    x.copy_(U.randn(g, rows, vocab, dtype=torch.bfloat16, scale=3.0))
+    dense = x.contiguous()
+    tok = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+    one = torch.ones(rows, device="cuda")
+    results = []
+    for t in (x, dense):
+        out = outputs(rows, 4, torch.bfloat16)
+        api.tokenLogProbs(U.ctx(), t, tok, *out)
+        dx = torch.empty_like(dense)
+        api.tokenLogProbsBackward(U.ctx(), t, tok, out[1], out[2], one, one, dx)
+        results.append(out + [dx])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    api.tokenLogProbsBackward(U.ctx(), x, tok, results[0][1], results[0][2], one, one, x)
+    assert torch.equal(x, results[0][-1])

@@ -255,3 +255,27 @@ def test_refusals():
     finally:
         c.set_scratch_limit(0)
     api.layerNormForward(c, x, w, w, x)                            # the context stays usable
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """Rows far apart: the last ones lie more than 2^31 elements from the first."""
+    rows, cols, ld = 33000, 64, 70000
+    g = U.gen(12)
+    base = torch.empty(rows * ld, device="cuda", dtype=torch.bfloat16)
+    x = base.as_strided((rows, cols), (ld, 1))
+    x.copy_(U.randn(g, rows, cols, dtype=torch.bfloat16))
+    dense = x.contiguous()
+    w = torch.ones(cols, device="cuda", dtype=torch.bfloat16)
+    c = U.ctx()
+    outs = []
+    for t in (x, dense):
+        y, mean, rstd = torch.empty_like(dense), torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+        api.layerNormForward(c, t, w, w, y, mean, rstd)
+        dx, dg, db = torch.empty_like(dense), torch.empty_like(w), torch.empty_like(w)
+        ws = torch.empty(api.layerNormBackwardMemRequired(rows, cols), device="cuda", dtype=torch.float64)
+        api.layerNormBackward(c, dense, t, w, mean, rstd, dx, dg, db, ws)
+        outs.append((y, mean, rstd, dx, dg, db))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    api.layerNormForward(c, x, w, w, x)                   # written there, too
+    assert torch.equal(x, outs[0][0])

@@ -255,3 +255,16 @@ def test_products_on_two_streams_at_once():
     for c in ctxs:
         c.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(alone, outs))
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    g = update(2, 70, 96, "full", torch.bfloat16)
+    apart = 1 << 31
+    far = torch.empty(apart + 70 * 96, device="cuda", dtype=torch.bfloat16).as_strided((2, 70, 96), (apart, 96, 1))
+    far.copy_(g)
+    want = run(g)
+    ws = torch.empty(api.orthogonalizeMemRequired(2, 70, 96), device="cuda", dtype=torch.float64)
+    api.orthogonalizeUpdate(U.ctx(), far, far, ws)
+    U.ctx().synchronize()
+    assert torch.equal(far, want)
