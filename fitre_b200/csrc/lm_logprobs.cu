@@ -262,6 +262,15 @@ token_logprobs_kernel(const T *__restrict__ logits, long ld, const long long *__
     const int edges = head + (hi - tail0);         // fewer than 2 * VEC, at most 14
     const T *xv = x + vbase;
 
+    // the given token's logit, fetched while the row is swept: two dependent loads that would end the row otherwise
+    A given = 0;
+    int state = 0;   // 1: the row has a token, -1: one out of range
+    if (logprobs && part == 0 && tid == 0) {
+        const long long tok = tokens[row];
+        state = tok >= vocab ? -1 : tok >= 0 ? 1 : 0;
+        if (state == 1) given = to_acc<A>(x[tok]);
+    }
+
     Running<A> run;
     Vec<T, VEC> raw[2][L_UNROLL];
     int at = tid;
@@ -327,11 +336,18 @@ token_logprobs_kernel(const T *__restrict__ logits, long ld, const long long *__
         if (tid < kMaxTop) blist[tid] = Entry<A>{-N::inf(), kNone};
     }
     __syncthreads();
-    if (tid == 0) {
-        Stats<A> r = wstat[0];
+    if (warp == WARPS - 1) {
+        Stats<A> r{N::lowest, 0, 0};
+        if (lane < WARPS) r = wstat[lane];
 #pragma unroll
-        for (int w = 1; w < WARPS; ++w) r = join(r, wstat[w]);
-        bstat = r;
+        for (int o = WARPS / 2; o > 0; o >>= 1) {
+            Stats<A> other;
+            other.m = __shfl_xor_sync(0xffffffffu, r.m, o);
+            other.s = __shfl_xor_sync(0xffffffffu, r.s, o);
+            other.t = __shfl_xor_sync(0xffffffffu, r.t, o);
+            r = (lane & o) ? join(other, r) : join(r, other);
+        }
+        if (lane == 0) bstat = r;
     }
     if (TOP) {
         // the bound: the top-th largest of what was put forward (every warp finds it for itself)
@@ -437,10 +453,9 @@ token_logprobs_kernel(const T *__restrict__ logits, long ld, const long long *__
                 if (lse_out) lse_out[row] = none ? -N::inf() : r.m + logs;
                 if (entropy) entropy[row] = none ? A(0) : logs - r.t / r.s;
                 if (logprobs) {
-                    const long long tok = tokens[row];
                     A lp = 0;
-                    if (tok >= vocab) lp = N::inf() - N::inf();
-                    else if (tok >= 0) lp = none ? -N::inf() : (to_acc<A>(x[tok]) - r.m) - logs;
+                    if (state < 0) lp = N::inf() - N::inf();
+                    else if (state) lp = none ? -N::inf() : (given - r.m) - logs;
                     logprobs[row] = lp;
                 }
             }
