@@ -17,6 +17,8 @@
 // 4 x 513 x 384 fp32 121 us (17 dependent kernels).
 // Products accumulate in fp32; the result is rounded to bf16 once, and is within about half a bf16
 // rounding of the exact polynomial before that.
+#include <cfloat>
+
 #include "lm_gemm.cuh"
 #include "lm_simd.cuh"
 
@@ -77,7 +79,9 @@ ortho_scale_kernel(const T *in, long ld, long bstride, int rows, int cols, int s
     __shared__ double s[8];
     double q = 0;
     for (int i = threadIdx.x; i < parts; i += 256) q += partial[(long)blockIdx.y * parts + i];
-    const double f = (double)kScale / (sqrt(block_sum(q, s)) + eps);
+    q = block_sum(q, s);
+    // squares that leave fp64's range (elements beyond 1e154): no number rather than zeros
+    const double f = q <= DBL_MAX ? (double)kScale / (sqrt(q) + eps) : nan("");
     const T *m = in + blockIdx.y * bstride;
     hi += blockIdx.y * ostride;
     lo += blockIdx.y * ostride;

@@ -729,7 +729,9 @@ int fitre_gated_backward(fitre_context *ctx, int dtype, int act, const void *dh,
  * side), out = scale * X in bf16.  coefficients_host: {a, b, c} on the host, NULL = {3.4445, -4.7750, 2.0315}.
  * The products take fp16 operands scaled by 2^10 and fp32 sums, the iterate itself is held to 22 bits: the
  * result is within about one bf16 rounding of the exact polynomial as long as the iteration keeps singular
- * values within about 30 and the coefficients' terms within 60 (it does with the default).  A zero matrix gives zero; one with a NaN or an infinity gives NaN.  out may be update.
+ * values within about 30 and the coefficients' terms within 60 (it does with the default).  A zero matrix gives zero,
+ * but NaN with eps = 0; so does, with any eps, one with a NaN or an infinity, or in fp64 one whose squares overflow their sum.
+ * out may be update.
  * devPtr: fitre_orthogonalize_mem_required doubles. */
 long fitre_orthogonalize_mem_required(long batch, long rows, long cols);
 int fitre_orthogonalize_update(fitre_context *ctx, int dtype, const void *update, long ldu, long strideu,

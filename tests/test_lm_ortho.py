@@ -122,6 +122,17 @@ def test_special_matrices():
 
 
 @gpu
+def test_the_range_of_fp64():
+    g = torch.stack([U.randn(U.gen(3), 20, 30).double().cuda() * f for f in (1e200, 1e150, 1e-150, 1e-200)])
+    out = run(g, eps=0.0)
+    assert torch.isnan(out[0]).all()                 # the sum of squares overflows
+    for i in (1, 2):
+        want = polynomial(g[i], eps=0.0)
+        assert (out[i].double() - want).norm() / want.norm() < 2 * BOUND
+    assert not run(g)[3].any()                       # far below eps
+
+
+@gpu
 def test_same_bits_on_a_stream_and_in_a_graph():
     g = update(2, 300, 520, "mixed", torch.float32)
     first = run(g)
