@@ -14,10 +14,11 @@
 // lower bound of the k-th largest element, so only the vectors of the few threads whose maximum reaches
 // it are read again (from L2) and filtered into lists that each warp keeps sorted across its lanes; lists
 // are joined by ranking their entries in one another.
+// Many short rows take a warp each instead of a block.
 // With few rows a cluster of up to 16 blocks shares a row and joins its statistics and lists over
 // distributed shared memory; no workspace, no atomics, one launch.
 // Backward: one read and one write of the logits, element by element.
-// Measured on a B200 (6.5 TB/s copy): 4096 x 128000 bf16 without alternatives 167 us (6.3 TB/s), with 8 of them 194 to 213
+// Measured on a B200 (6.5 TB/s copy): 4096 x 128000 bf16 without alternatives 165 us (6.4 TB/s), with 8 of them 196 to 213
 // us (264 us without the packed sweep and the closer bound); 8 x 128000 with 20 of them 10 us; the gradient
 // over 4099 x 50001 143 us (5.7 TB/s; 170 us with scalar arithmetic).
 #include <cooperative_groups.h>
@@ -473,6 +474,111 @@ token_logprobs_kernel(const T *__restrict__ logits, long ld, const long long *__
     if (parts > 1) cluster.sync();                 // the other blocks' shared memory was read above
 }
 
+// Short rows: a warp per row, no barrier and no shared memory.  The same sweep; the lanes' maxima bound the alternatives.
+template <class T, bool TOP>
+__global__ void __launch_bounds__(256, sweep_threads<T> / 256)
+token_logprobs_warp_kernel(const T *__restrict__ logits, long ld, const long long *__restrict__ tokens, long rows, int vocab,
+                           int top, acc_t<T> *logprobs, acc_t<T> *lse_out, acc_t<T> *entropy, acc_t<T> *top_logprobs,
+                           long long *top_tokens) {
+    using A = acc_t<T>;
+    using N = Num<A>;
+    constexpr int VEC = 16 / sizeof(T), STEP = 32 * L_UNROLL;
+    const int lane = threadIdx.x & 31;
+    const long row = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    const T *x = logits + row * ld;
+    int head = (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T);
+    head = head < vocab ? head : vocab;
+    const int nvec = (vocab - head) / VEC, tail0 = head + nvec * VEC, edges = head + (vocab - tail0);
+    const T *xv = x + head;
+    A given = 0;
+    int state = 0;   // 1: the row has a token, -1: one out of range
+    if (logprobs && lane == 0) {
+        const long long tok = tokens[row];
+        state = tok >= vocab ? -1 : tok >= 0 ? 1 : 0;
+        if (state == 1) given = to_acc<A>(x[tok]);
+    }
+    const int edge_at = lane < head ? lane : tail0 + (lane - head);
+    A edge_v = -N::inf();
+    if (lane < edges) edge_v = to_acc<A>(x[edge_at]);
+
+    Running<A> run;
+    int at = lane;
+    for (; at - lane + STEP <= nvec; at += STEP) {
+        Vec<T, VEC> raw[L_UNROLL];
+#pragma unroll
+        for (int u = 0; u < L_UNROLL; ++u) raw[u] = load_vec<T, VEC>(xv + (long)(at + u * 32) * VEC);
+        A m = vec_max(raw[0]);
+#pragma unroll
+        for (int u = 1; u < L_UNROLL; ++u) m = N::max(m, vec_max(raw[u]));
+        run.follow(m);
+        run.template vectors<L_UNROLL>(raw);
+    }
+    {
+        Vec<T, VEC> raw[L_UNROLL];
+#pragma unroll
+        for (int u = 0; u < L_UNROLL; ++u)
+            if (at + u * 32 < nvec) raw[u] = load_vec<T, VEC>(xv + (long)(at + u * 32) * VEC);
+#pragma unroll
+        for (int u = 0; u < L_UNROLL; ++u)
+            if (at + u * 32 < nvec) {
+                run.follow(vec_max(raw[u]));
+                run.template vectors<1>(&raw[u]);
+            }
+    }
+    if (lane < edges) {
+        run.follow(edge_v);
+        run.element(edge_v);
+    }
+    Stats<A> r{warp_max(run.st.m), 0, 0};
+    r = join(r, run.st);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
+        r.t += __shfl_xor_sync(0xffffffffu, r.t, o);
+    }
+    const bool none = r.s == A(0);                 // every logit is -inf: no distribution
+    const A logs = N::log_(r.s);
+    if (lane == 0) {
+        if (lse_out) lse_out[row] = none ? -N::inf() : r.m + logs;
+        if (entropy) entropy[row] = none ? A(0) : logs - r.t / r.s;
+        if (logprobs) {
+            A lp = 0;
+            if (state < 0) lp = N::inf() - N::inf();
+            else if (state) lp = none ? -N::inf() : (given - r.m) - logs;
+            logprobs[row] = lp;
+        }
+    }
+    if (TOP) {
+        int rank = 0;
+        for (int o = 0; o < 32; ++o) rank += better(__shfl_sync(0xffffffffu, run.top, o), o, run.top, lane) ? 1 : 0;
+        const A bound = __shfl_sync(0xffffffffu, run.top, __ffs(__ballot_sync(0xffffffffu, rank == top - 1)) - 1);
+        WarpList<A> list(top, lane);
+        if (edge_v != edge_v) edge_v = -N::inf();  // a NaN ranks as -inf
+        list.offer(lane < edges && edge_v >= bound, edge_v, edge_at);
+        for (int v0 = 0; v0 < nvec; v0 += 32) {
+            Vec<T, VEC> raw;
+            bool worth = v0 + lane < nvec && run.top >= bound;
+            if (worth) {
+                raw = load_vec<T, VEC>(xv + (long)(v0 + lane) * VEC);
+                worth = vec_max(raw) >= bound || bound == -N::inf();
+            }
+            if (__any_sync(0xffffffffu, worth))
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    A v = worth ? to_acc<A>(raw.v[e]) : -N::inf();
+                    if (v != v) v = -N::inf();
+                    const bool has = worth && v >= bound;
+                    if (__any_sync(0xffffffffu, has)) list.offer(has, v, head + (v0 + lane) * VEC + e);
+                }
+        }
+        if (lane < top) {
+            top_tokens[row * top + lane] = list.e.i;
+            top_logprobs[row * top + lane] = none ? -N::inf() : (list.e.v - r.m) - logs;
+        }
+    }
+}
+
 constexpr int B_UNROLL = 4;
 
 template <class T, int THREADS, int VEC>
@@ -575,6 +681,15 @@ void launch_logprobs(fitre_context *ctx, const LogProbArgs &a, int parts) {
     check_launch(ctx, "token_logprobs_kernel");
 }
 
+template <class T, bool TOP>
+void launch_short(fitre_context *ctx, const LogProbArgs &a) {
+    using A = acc_t<T>;
+    token_logprobs_warp_kernel<T, TOP><<<(unsigned)((a.rows + 7) / 8), 256, 0, ctx->stream>>>(
+        (const T *)a.logits, a.ld, a.tokens, a.rows, a.vocab, a.top, (A *)a.logprobs, (A *)a.lse, (A *)a.entropy,
+        (A *)a.top_logprobs, a.top_tokens);
+    check_launch(ctx, "token_logprobs_warp_kernel");
+}
+
 // Blocks that share a row: more while the rows alone leave SMs idle, but no slice under 4096 logits.
 int parts_for(long rows, int vocab) {
     int parts = 1;
@@ -582,14 +697,27 @@ int parts_for(long rows, int vocab) {
     return parts;
 }
 
+// Whether a warp takes a row.  It does where rows are short and enough for 16 warps per SM: what a block spends on its start
+// and its barriers is then more than the sweep (150000 x 2000 bf16 without alternatives 174 us, 452 us in blocks; 1000 x
+// 8192 9 us either way).  Alternatives are inserted one by one, which blocks do better when rows are longer or there are
+// many (top 8: 36621 x 8192 bf16 207 and 264 us, 18310 x 16384 251 and 194 us; top 32: 4000 x 1003 38 us either way).
+bool short_rows(const LogProbArgs &a, long row_bytes) {
+    return a.rows >= 16 * kLmSms && (a.top ? row_bytes <= 16384 && row_bytes * a.top <= 131072 : row_bytes <= 32768);
+}
+
 template <class T>
 void logprobs_as(fitre_context *ctx, const LogProbArgs &a) {
+    const long row_bytes = (long)a.vocab * sizeof(T);
+    if (short_rows(a, row_bytes)) return a.top ? launch_short<T, true>(ctx, a) : launch_short<T, false>(ctx, a);
     const int parts = parts_for(a.rows, a.vocab);
-    const bool narrow = a.vocab <= 4096;   // a short row keeps 64 threads busy, not 256
+    // 128 threads for short rows, and for longer ones that are more than 256-thread blocks fit the GPU: twice the rows in
+    // flight hide the phases behind the sweep (bf16, top 8: 12500 x 32000 203 and 229 us, 6250 x 64000 173 and 175 us, 3125
+    // x 128000 178 and 155 us; 300 x 50000 17 us either way)
+    const bool narrow = a.vocab <= 4096 || (a.rows > 4 * kLmSms && row_bytes <= 112 * 1024);
     if (a.top) {
-        narrow ? launch_logprobs<T, 64, true>(ctx, a, parts) : launch_logprobs<T, 256, true>(ctx, a, parts);
+        narrow ? launch_logprobs<T, 128, true>(ctx, a, parts) : launch_logprobs<T, 256, true>(ctx, a, parts);
     } else {
-        narrow ? launch_logprobs<T, 64, false>(ctx, a, parts) : launch_logprobs<T, 256, false>(ctx, a, parts);
+        narrow ? launch_logprobs<T, 128, false>(ctx, a, parts) : launch_logprobs<T, 256, false>(ctx, a, parts);
     }
 }
 

@@ -79,6 +79,66 @@ def test_forward(shape, kind):
 
 
 @gpu
+@pytest.mark.parametrize("shape", [(2400, 1), (2401, 5), (2500, 33), (2368, 255), (3001, 1024), (2371, 2049), (2400, 4097),
+                                   (2390, 8192), (2368, 16001), (600, 30003)], ids=str)
+@pytest.mark.parametrize("kind", ["f64", "f32", "bf16", "f16"])
+def test_many_short_rows(shape, kind):
+    # a warp per row adds chains of vocab / 32 elements, in pairs (fp64: up to 4096 elements, singly): within `chain`
+    dtype = U.TYPES[kind]
+    rows, vocab = shape
+    g = U.gen(rows + vocab)
+    x = U.randn(g, rows, vocab, dtype=dtype, scale=3.0)
+    x[5, vocab // 2:] = -INF
+    x[7] = torch.finfo(dtype).min
+    x[8, 0] = 50.0
+    tokens = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+    tokens[5] = 0
+    tokens[rows // 2] = vocab - 1
+    tokens[1] = -1
+    if vocab == 1:
+        x[5] = 1.0
+    for top in sorted({0, 1, *(min(t, max(1, vocab // 2)) for t in (3, 8, 32))}):
+        for how in ("dense", "strided", "odd"):
+            out = outputs(rows, top, dtype)
+            api.tokenLogProbs(U.ctx(), U.laid_out(x, how), tokens, *out)
+            check(x, tokens, out, dtype, top)
+
+
+@gpu
+@pytest.mark.parametrize("vocab", [40, 1000, 7000])
+@pytest.mark.parametrize("kind", ["f64", "f32", "bf16", "f16"])
+def test_many_short_rows_without_a_distribution(vocab, kind):
+    dtype = U.TYPES[kind]
+    rows = 2400
+    x = U.randn(U.gen(vocab), rows, vocab, dtype=dtype)
+    tokens = torch.full((rows,), 3, device="cuda")
+    x[0] = -INF
+    x[1, 6] = float("nan")
+    x[2, vocab - 1] = INF
+    tokens[3] = vocab
+    x[4] = 0.0                                                 # ties: the lower index first
+    x[5] = -INF
+    x[5, 9] = -1.0
+    for top in (0, 2, min(8, vocab)):
+        out = outputs(rows, top, dtype)
+        api.tokenLogProbs(U.ctx(), x, tokens, *out)
+        lp, lse, ent = (o[:6].tolist() for o in out[:3])
+        assert lse[0] == -INF and lp[0] == -INF and ent[0] == 0
+        assert all(v != v for i in (1, 2) for v in (lp[i], lse[i], ent[i]))
+        assert lp[3] != lp[3] and lse[3] == lse[3]
+        assert lse[5] == -1.0 and ent[5] == 0 and lp[5] == -INF
+        if top:
+            order = list(range(top))
+            assert out[4][0].tolist() == order and (out[3][0] == -INF).all()
+            assert out[4][4].tolist() == order
+            assert 6 not in out[4][1].tolist()
+            assert out[4][2, 0] == vocab - 1
+            assert out[4][5].tolist() == [9] + order[:-1] and (out[3][5, 1:] == -INF).all()
+        rest = slice(6, None)
+        check(x[rest], tokens[rest], [None if o is None else o[rest] for o in out], dtype, top)
+
+
+@gpu
 @pytest.mark.parametrize("vocab", [64, 999, 40000])
 def test_ties_order_and_extremes(vocab):
     dtype = torch.float32
