@@ -16,11 +16,11 @@
 // are joined by ranking their entries in one another.
 // Many short rows take a warp each instead of a block.
 // With few rows a cluster of up to 16 blocks shares a row and joins its statistics and lists over
-// distributed shared memory; no workspace, no atomics, one launch.
+// distributed shared memory; no workspace, one launch.
 // Backward: one read and one write of the logits, element by element.
-// Measured on a B200 (6.5 TB/s copy): 4096 x 128000 bf16 without alternatives 165 us (6.4 TB/s), with 8 of them 196 to 213
+// Measured on a B200 (6.5 TB/s copy): 4096 x 128000 bf16 without alternatives 165 us (6.4 TB/s), with 8 of them 196 to 215
 // us (264 us without the packed sweep and the closer bound); 8 x 128000 with 20 of them 10 us; the gradient
-// over 4099 x 50001 143 us (5.7 TB/s; 170 us with scalar arithmetic).
+// over 4099 x 50001 140 us (5.9 TB/s; 170 us with scalar arithmetic).
 #include <cooperative_groups.h>
 
 #include <cfloat>
@@ -739,12 +739,9 @@ void backward_as(fitre_context *ctx, const LogProbArgs &a) {
     // vectors need every row of both matrices at the same distance from a 16-byte boundary
     const bool same = (((uintptr_t)a.logits ^ (uintptr_t)a.dlogits) & 15) == 0 &&
                       (a.rows == 1 || ((a.ld - a.ldd) * (long)sizeof(T)) % 16 == 0);
-    const bool narrow = a.vocab <= 64 * B_UNROLL * VEC;
-    if (same) {
-        narrow ? launch_backward<T, 64, VEC>(ctx, a) : launch_backward<T, 256, VEC>(ctx, a);
-    } else {
-        narrow ? launch_backward<T, 64, 1>(ctx, a) : launch_backward<T, 256, 1>(ctx, a);
-    }
+    // small blocks: their shares come out full at more widths (bf16, 64 and 256 threads: 49962 x 4003 130 and 175 us, 19998 x
+    // 10001 132 and 160 us, 1562 x 128000 126 and 128 us)
+    same ? launch_backward<T, 64, VEC>(ctx, a) : launch_backward<T, 64, 1>(ctx, a);
 }
 
 }  // namespace
