@@ -579,9 +579,7 @@ token_logprobs_warp_kernel(const T *__restrict__ logits, long ld, const long lon
     }
 }
 
-constexpr int B_UNROLL = 4;
-
-template <class T, int THREADS, int VEC>
+template <class T, int THREADS, int VEC, int B_UNROLL>
 __global__ void __launch_bounds__(THREADS)
 token_logprobs_backward_kernel(const T *logits, long ld, const long long *__restrict__ tokens,
                                const acc_t<T> *__restrict__ lse, const acc_t<T> *__restrict__ entropy,
@@ -721,13 +719,13 @@ void logprobs_as(fitre_context *ctx, const LogProbArgs &a) {
     }
 }
 
-template <class T, int THREADS, int VEC>
+template <class T, int THREADS, int VEC, int B_UNROLL>
 void launch_backward(fitre_context *ctx, const LogProbArgs &a) {
     using A = acc_t<T>;
     const int per = THREADS * B_UNROLL * VEC;
     const int chunks = (a.vocab + per - 1) / per;
     FITRE_REQUIRE(a.rows <= 0x7fffffffl / chunks, FITRE_ERR_TOO_LARGE, "token log probabilities: too many logits");
-    token_logprobs_backward_kernel<T, THREADS, VEC><<<(unsigned)(a.rows * chunks), THREADS, 0, ctx->stream>>>(
+    token_logprobs_backward_kernel<T, THREADS, VEC, B_UNROLL><<<(unsigned)(a.rows * chunks), THREADS, 0, ctx->stream>>>(
         (const T *)a.logits, a.ld, a.tokens, (const A *)a.lse, (const A *)a.entropy, (const A *)a.dlogprobs,
         (const A *)a.dentropy, (T *)a.dlogits, a.ldd, a.vocab, chunks);
     check_launch(ctx, "token_logprobs_backward_kernel");
@@ -740,8 +738,9 @@ void backward_as(fitre_context *ctx, const LogProbArgs &a) {
     const bool same = (((uintptr_t)a.logits ^ (uintptr_t)a.dlogits) & 15) == 0 &&
                       (a.rows == 1 || ((a.ld - a.ldd) * (long)sizeof(T)) % 16 == 0);
     // small blocks: their shares come out full at more widths (bf16, 64 and 256 threads: 49962 x 4003 130 and 175 us, 19998 x
-    // 10001 132 and 160 us, 1562 x 128000 126 and 128 us)
-    same ? launch_backward<T, 64, VEC>(ctx, a) : launch_backward<T, 64, 1>(ctx, a);
+    // 10001 132 and 160 us, 1562 x 128000 126 and 128 us).  Single elements, 16 to a thread: 6250 x 32000 248 us, 343 us with 4
+    // in blocks of 256.
+    same ? launch_backward<T, 64, VEC, 4>(ctx, a) : launch_backward<T, 64, 1, 16>(ctx, a);
 }
 
 }  // namespace
